@@ -54,7 +54,13 @@ def _headers_bytes():
     return out
 
 
-def object_digest(src, flags=(ARCH, "-O3"), headers=None):
+# Packed fp32 arithmetic (v_pk_add/mul/fma_f32) stays off: some of its forms have given wrong
+# results on gfx950 without an error, and -O3 makes them from ordinary float code by itself.  The
+# host pass does not know the feature and warns, which is harmless.
+NO_PACKED_FP32 = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
+
+
+def object_digest(src, flags=(ARCH, "-O3") + NO_PACKED_FP32, headers=None):
     """sha256 of ONE translation unit's inputs: its bytes, every local header and the
     compile flags.  Stored beside the object (``<obj>.srchash``); an object is reused only
     when this digest matches (not by mtime: a copy that preserves times cannot pass off
@@ -109,6 +115,7 @@ def _compile(src, inc, abi, force):
         "-DUSE_ROCM",
         "-Wno-unused-result",
         "-Wno-deprecated-declarations",
+        *NO_PACKED_FP32,
         f"-I{HERE}",
         f"-I{py_inc}",
     ] + [f"-I{p}" for p in inc] + ["-c", src, "-o", obj]
