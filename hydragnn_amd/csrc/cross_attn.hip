@@ -1,0 +1,178 @@
+// Ragged cross attention: the operators' entries (arguments, outputs, workspaces).
+#include <c10/core/DeviceGuard.h>
+
+#include "cross_attn.h"
+
+namespace hy {
+namespace xa {
+
+void forward(const Args& a, at::ScalarType t, int bias, hipStream_t st);
+void backward(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st);
+int64_t table_tiles(int64_t Nq, int64_t S, at::ScalarType t);
+
+typedef c10::optional<at::Tensor> OptTensor;
+
+// rows of `t` [N, H, D] may be read 16 bytes at a time
+static int vec16(const at::Tensor& t, int64_t D) {
+  const int64_t per = 16 / t.element_size();
+  return D % per == 0 && t.stride(0) % per == 0 && t.stride(1) % per == 0 && ((uintptr_t)t.data_ptr() & 15) == 0;
+}
+
+static at::Tensor rows(const at::Tensor& t) { return t.stride(2) == 1 || t.size(2) <= 1 ? t : t.contiguous(); }
+
+// rule: [two_sided, side, near, far, thresholds...]
+static int fill(Args& a, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& q_ptr,
+                const at::Tensor& k_ptr, const OptTensor& mask, double scale, const OptTensor& table,
+                const OptTensor& q_pos, const OptTensor& k_pos, at::IntArrayRef rule, double unit) {
+  HY_CHECK_CUDA(q);
+  const auto dev = q.device();
+  const auto t = q.scalar_type();
+  HY_CHECK(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "cross_attention: q must be fp32, bf16 or fp16");
+  HY_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes(), "cross_attention: q, k, v shapes");
+  HY_CHECK(k.scalar_type() == t && v.scalar_type() == t, "cross_attention: q, k and v must have one type");
+  const int64_t H = q.size(1), Hk = k.size(1), D = q.size(2);
+  HY_CHECK(k.size(2) == D && D >= 1 && D <= 128, "cross_attention: one head width of 1 to 128");
+  HY_CHECK(Hk >= 1 && H >= 1 && H % Hk == 0, "cross_attention: query heads must be a multiple of the key heads");
+  HY_CHECK(q.size(0) < INT_MAX / 2 && k.size(0) < INT_MAX / 2, "cross_attention: too many rows");
+  for (const auto& p : {q_ptr, k_ptr}) {
+    HY_CHECK(p.device() == dev && p.is_contiguous() && p.scalar_type() == at::kInt && p.dim() == 1 && p.numel() >= 1 &&
+                 p.numel() == q_ptr.numel(),
+             "cross_attention: q_ptr and k_ptr must be contiguous int32 of one length on q's device");
+  }
+  HY_CHECK(k.device() == dev && v.device() == dev, "cross_attention: tensors on several devices");
+  a.Nq = (int)q.size(0);
+  a.Nk = (int)k.size(0);
+  a.S = (int)q_ptr.numel() - 1;
+  a.H = (int)H;
+  a.Hk = (int)Hk;
+  a.G = (int)(H / Hk);
+  a.D = (int)D;
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.q_row = q.stride(0), a.q_head = q.stride(1);
+  a.k_row = k.stride(0), a.k_head = k.stride(1);
+  a.v_row = v.stride(0), a.v_head = v.stride(1);
+  a.vec_q = vec16(q, D), a.vec_k = vec16(k, D), a.vec_v = vec16(v, D);
+  a.q_ptr = q_ptr.data_ptr<int>();
+  a.k_ptr = k_ptr.data_ptr<int>();
+  a.scale = (float)scale;
+  a.key_mask = nullptr;
+  if (mask.has_value()) {
+    HY_CHECK(mask->device() == dev && mask->scalar_type() == at::kBool && mask->is_contiguous() &&
+                 mask->numel() == k.size(0),
+             "cross_attention: key_mask must be a contiguous bool for each key row");
+    a.key_mask = (const uint8_t*)mask->data_ptr();
+  }
+  if (!table.has_value()) return kNoBias;
+  HY_CHECK(q_pos.has_value() && k_pos.has_value(), "cross_attention: a table needs q_pos and k_pos");
+  const int bias = unit > 0 ? kSpace : kOrder;
+  const auto pt = bias == kSpace ? at::kFloat : at::kInt;
+  const int64_t w = bias == kSpace ? 3 : 1;
+  HY_CHECK(table->device() == dev && table->scalar_type() == at::kFloat && table->is_contiguous() && table->dim() == 2 &&
+               table->size(0) == H && table->size(1) >= 1 && table->size(1) <= kMaxBuckets,
+           "cross_attention: table must be contiguous fp32 [heads, buckets]");
+  HY_CHECK(q_pos->device() == dev && k_pos->device() == dev && q_pos->scalar_type() == pt &&
+               k_pos->scalar_type() == pt && q_pos->is_contiguous() && k_pos->is_contiguous() &&
+               q_pos->numel() == w * q.size(0) && k_pos->numel() == w * k.size(0),
+           "cross_attention: positions must be contiguous, int32 [rows] or fp32 [rows, 3]");
+  HY_CHECK(rule.size() >= 4 && rule.size() <= 4 + kMaxBuckets, "cross_attention: bucket rule");
+  Rule& r = a.rule;
+  r.buckets = (int)table->size(1);
+  r.two_sided = (int)rule[0];
+  r.side = (int)rule[1];
+  r.near = (int)rule[2];
+  r.far = (int)rule[3];
+  r.nthr = (int)rule.size() - 4;
+  for (int i = 0; i < r.nthr; ++i) r.thr[i] = (int)rule[4 + i];
+  HY_CHECK(r.near >= 1 && r.far >= 1 && r.far <= kMaxFar && r.side == r.near + r.nthr + 1 &&
+               r.buckets == r.side * (r.two_sided ? 2 : 1) && !(r.two_sided && bias == kSpace),
+           "cross_attention: bucket rule");
+  r.unit = unit;
+  r.inv_unit = bias == kSpace ? (float)(1.0 / unit) : 0.f;
+  a.table = table->data_ptr();
+  a.q_pos = q_pos->data_ptr();
+  a.k_pos = k_pos->data_ptr();
+  return bias;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_fwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
+                                                  const at::Tensor& q_ptr, const at::Tensor& k_ptr,
+                                                  const OptTensor& mask, double scale, const OptTensor& table,
+                                                  const OptTensor& q_pos, const OptTensor& k_pos, at::IntArrayRef rule,
+                                                  double unit, bool save) {
+  HY_CHECK_CUDA(q_);
+  c10::DeviceGuard guard(q_.device());
+  const at::Tensor q = rows(q_), k = rows(k_), v = rows(v_);
+  Args a = {};
+  const int bias = fill(a, q, k, v, q_ptr, k_ptr, mask, scale, table, q_pos, k_pos, rule, unit);
+  at::Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  at::Tensor lse = at::empty({save ? a.H : 0, save ? a.Nq : 0}, q.options().dtype(at::kFloat));
+  at::Tensor rest = at::empty({save && q.scalar_type() != at::kFloat ? out.numel() : 0}, q.options());
+  if (a.Nq == 0) return {out, rest, lse};
+  a.rest = rest.numel() > 0 ? rest.data_ptr() : nullptr;
+  a.out = out.data_ptr();
+  a.lse = save ? lse.data_ptr<float>() : nullptr;
+  forward(a, q.scalar_type(), bias, stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return {out, rest, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd(
+    const at::Tensor& d_out, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& out,
+    const at::Tensor& rest, const at::Tensor& lse, const at::Tensor& q_ptr, const at::Tensor& k_ptr, const OptTensor& mask, double scale,
+    const OptTensor& table, const OptTensor& q_pos, const OptTensor& k_pos, at::IntArrayRef rule, double unit) {
+  HY_CHECK_CUDA(q_);
+  c10::DeviceGuard guard(q_.device());
+  const at::Tensor q = rows(q_), k = rows(k_), v = rows(v_);
+  HY_CHECK(d_out.sizes() == q.sizes() && d_out.scalar_type() == q.scalar_type() && d_out.device() == q.device(),
+           "cross_attention: the output's gradient must be like the output");
+  const at::Tensor dout = rows(d_out);
+  Args a = {};
+  const int bias = fill(a, q, k, v, q_ptr, k_ptr, mask, scale, table, q_pos, k_pos, rule, unit);
+  HY_CHECK(out.sizes() == q.sizes() && out.is_contiguous() && lse.is_contiguous() &&
+               lse.numel() == (int64_t)a.H * a.Nq && lse.scalar_type() == at::kFloat &&
+               rest.numel() == (q.scalar_type() == at::kFloat ? 0 : out.numel()) && rest.is_contiguous() &&
+               rest.scalar_type() == q.scalar_type(),
+           "cross_attention: saved outputs");
+  const auto f32 = q.options().dtype(at::kFloat);
+  at::Tensor dq = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  at::Tensor dk = at::empty({k.size(0), k.size(1), k.size(2)}, q.options());
+  at::Tensor dv = at::empty({k.size(0), k.size(1), k.size(2)}, q.options());
+  at::Tensor dtable = bias != kNoBias ? at::empty({a.H, a.rule.buckets}, f32) : at::empty({0}, f32);
+  at::Tensor delta = at::empty({a.H, a.Nq}, f32);
+  at::Tensor part = bias != kNoBias
+                        ? at::empty({table_tiles(a.Nq, a.S, q.scalar_type()) * a.H * a.rule.buckets}, f32)
+                        : at::Tensor();
+  a.out = out.data_ptr();
+  a.rest = rest.numel() > 0 ? rest.data_ptr() : nullptr;
+  a.lse = lse.data_ptr<float>();
+  a.d_out = dout.data_ptr();
+  a.do_row = dout.stride(0), a.do_head = dout.stride(1);
+  a.vec_do = vec16(dout, a.D);
+  a.delta = delta.data_ptr<float>();
+  a.dq = dq.data_ptr();
+  a.dk = dk.data_ptr();
+  a.dv = dv.data_ptr();
+  a.part = bias != kNoBias ? part.data_ptr<float>() : nullptr;
+  backward(a, q.scalar_type(), bias, bias != kNoBias ? dtable.data_ptr<float>() : nullptr, stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return {dq, dk, dv, dtable};
+}
+
+}  // namespace xa
+}  // namespace hy
+
+TORCH_LIBRARY_FRAGMENT(hydra, m) {
+  m.def(
+      "cross_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor q_ptr, Tensor k_ptr, Tensor? key_mask, float scale, "
+      "Tensor? table, Tensor? q_pos, Tensor? k_pos, int[] rule, float unit, bool save) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "cross_attn_bwd(Tensor d_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor rest, Tensor lse, Tensor q_ptr, Tensor k_ptr, "
+      "Tensor? key_mask, float scale, Tensor? table, Tensor? q_pos, Tensor? k_pos, int[] rule, float unit) -> "
+      "(Tensor, Tensor, Tensor, Tensor)");
+}
+TORCH_LIBRARY_IMPL(hydra, CUDA, m) {
+  m.impl("cross_attn_fwd", hy::xa::cross_attn_fwd);
+  m.impl("cross_attn_bwd", hy::xa::cross_attn_bwd);
+}

@@ -1,0 +1,702 @@
+// Group norm over the rows of each sequence, channels last, with an activation, both ways.
+//
+//   z = (x - mean) inv w + b,  y = act(z),  inv = 1 / sqrt(var + eps)
+//
+// mean and var go over the rows of a sequence and the C / G channels of a group.  With
+// dz = dy act'(z), xh = (x - mean) inv, and M(.) the mean over a sequence's group:
+//
+//   dx = inv (w dz - M(w dz) - xh M(w dz xh)),  dw = sum over all rows of dz xh,  db = of dz
+//
+// Bound by memory: forward reads x twice (the second time from the caches where a sequence fits
+// them) and writes y; backward reads x and dy twice and writes dx.  A thread keeps the same 16
+// bytes of channels for all its rows, so the channels' parameters and sums stay in registers.
+//
+// Two forms by size alone (group_norm.hip's `whole`): one workgroup a sequence for short ones (one
+// launch), and chunks of rows whose sums a second launch joins in order for long ones.  Sums of x
+// are held in 64 bits, because E[x^2] - E[x]^2 loses what the mean exceeds the deviation by; no sum
+// goes by atomics.
+#include <c10/core/DeviceGuard.h>
+
+#include "ragged.h"
+
+namespace hy {
+namespace gn {
+
+constexpr int kThreads = 256;
+
+struct Args {
+  const void *x, *dy;
+  int64_t x_row, dy_row;
+  void *y, *dx;  // contiguous [N, C]
+  const float *w, *b;  // may be null
+  const int* ptr;      // null: sequences of `uniform` rows
+  int64_t uniform;
+  int N, S, C, G, chunk;
+  float eps;
+  float* stat;   // [S, G, 2]: mean, inv
+  double* part;  // [chunks, G, 2]
+  float* cpart;  // [chunks, C, 2]: db, dw of a chunk
+  float *dw, *db;
+  int chunks;
+};
+
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int kPer = 4;
+};
+template <>
+struct Vec<__bf16> {
+  static constexpr int kPer = 8;
+};
+template <>
+struct Vec<_Float16> {
+  static constexpr int kPer = 8;
+};
+
+enum Act { kNone = 0, kRelu = 1, kSilu = 2 };
+
+__device__ __forceinline__ float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+}
+
+template <int ACT>
+__device__ __forceinline__ float act(float z) {
+  if constexpr (ACT == kRelu) return z > 0.f || z != z ? z : 0.f;
+  if constexpr (ACT == kSilu) return z * sigmoid(z);
+  return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_grad(float z) {
+  if constexpr (ACT == kRelu) return z > 0.f ? 1.f : 0.f;
+  if constexpr (ACT == kSilu) {
+    const float s = sigmoid(z);
+    return s * (1.f + z * (1.f - s));
+  }
+  return 1.f;
+}
+
+// PER channels from c on; VEC: 16 bytes at once (the host has looked at alignment and C)
+template <typename T, int PER, bool VEC>
+__device__ __forceinline__ void load(const T* p, int c, int C, float (&v)[PER]) {
+  if constexpr (VEC) {
+    union {
+      uint4 u;
+      T e[PER];
+    } r;
+    r.u = *reinterpret_cast<const uint4*>(p + c);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = (float)r.e[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = c + i < C ? (float)p[c + i] : 0.f;
+  }
+}
+
+template <typename T, int PER, bool VEC>
+__device__ __forceinline__ void store(T* p, int c, int C, const float (&v)[PER]) {
+  if constexpr (VEC) {
+    union {
+      uint4 u;
+      T e[PER];
+    } r;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) r.e[i] = (T)v[i];
+    *reinterpret_cast<uint4*>(p + c) = r.u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (c + i < C) p[c + i] = (T)v[i];
+  }
+}
+
+// w dz rounded to 32 bits wherever it is formed: a group of a single value has then no gradient at
+// all, where a fused multiply and subtract would leave the product's rounding over the deviation.
+__device__ __forceinline__ float product(float w, float dz) {
+#pragma clang fp contract(off)
+  const float t = w * dz;
+  return t;
+}
+
+// Where a workgroup's threads stand: tx of the channels' vectors, ty of the rows
+struct Place {
+  int tx, ty, nx, ny;
+};
+
+__device__ __forceinline__ Place place(int C, int per) {
+  const int vecs = (C + per - 1) / per;
+  Place p;
+  p.nx = min(vecs, kThreads);
+  p.ny = kThreads / p.nx;
+  p.ty = threadIdx.x / p.nx;
+  p.tx = threadIdx.x - p.ty * p.nx;
+  return p;
+}
+
+// Sums of `vals[2]` of each of G groups over `items` entries: P threads a group, fixed order.
+// get(group, item, out[2]); put(group, sums[2]).
+template <typename V, typename Get, typename Put>
+__device__ __forceinline__ void group_sums(int G, int items, Get get, Put put) {
+  int P = 64;
+  while (P > 1 && P * G > kThreads) P >>= 1;
+  const int sub = threadIdx.x & (P - 1);
+  for (int g0 = 0; g0 < G; g0 += kThreads / P) {
+    const int g = g0 + threadIdx.x / P;
+    V s0 = 0, s1 = 0;
+    if (g < G)
+      for (int i = sub; i < items; i += P) {
+        V t[2];
+        get(g, i, t);
+        s0 += t[0];
+        s1 += t[1];
+      }
+    for (int o = P >> 1; o > 0; o >>= 1) {
+      s0 += __shfl_xor(s0, o, 64);
+      s1 += __shfl_xor(s1, o, 64);
+    }
+    if (g < G && sub == 0) put(g, s0, s1);
+  }
+}
+
+__device__ __forceinline__ int start_of(const Args& a, int e) {
+  if (a.ptr != nullptr) return ptr_at(a.ptr, a.S, a.N, e);
+  return e == 0 ? 0 : e == a.S + 2 ? a.N : (int)min((int64_t)(e - 1) * a.uniform, (int64_t)a.N);
+}
+
+// Rows of this workgroup: a whole sequence (WHOLE; e = blockIdx.x, as in find_tile) or one chunk.
+struct Rows {
+  int seq, start, end;    // of this workgroup
+  int first, chunks;      // the sequence's chunks
+  int length;             // rows of the sequence
+};
+
+template <bool WHOLE>
+__device__ __forceinline__ Rows my_rows(const Args& a) {
+  Rows r;
+  int e;
+  if constexpr (WHOLE) {
+    e = blockIdx.x;
+  } else {  // as find_tile, by bisection over either kind of pointers
+    int lo = 0, hi = a.S + 2;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start_of(a, mid) / a.chunk + mid <= (int)blockIdx.x) lo = mid;
+      else hi = mid;
+    }
+    e = lo;
+  }
+  const int s0 = start_of(a, e), s1 = max(start_of(a, e + 1), s0);
+  r.seq = e >= 1 && e <= a.S ? e - 1 : -1;
+  r.length = s1 - s0;
+  if constexpr (WHOLE) {
+    r.start = s0;
+    r.end = s1;
+    r.first = 0;
+    r.chunks = 1;
+  } else {
+    r.first = s0 / a.chunk + e;
+    r.chunks = (r.length + a.chunk - 1) / a.chunk;
+    const int64_t off = (int)blockIdx.x - r.first, at = s0 + off * a.chunk;
+    r.start = off >= 0 && at < s1 ? (int)at : s1;  // (off < 0: pointers that do not ascend)
+    r.end = min(s1 - r.start, a.chunk) + r.start;
+  }
+  return r;
+}
+
+template <typename T, int PER, bool VEC>
+__device__ void zero_rows(T* out, const Rows& r, int C, const Place& p) {
+  float z[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) z[i] = 0.f;
+  if (p.ty < p.ny)
+    for (int row = r.start + p.ty; row < r.end; row += p.ny)
+      for (int c = p.tx * PER; c < C; c += p.nx * PER) store<T, PER, VEC>(out + (int64_t)row * C, c, C, z);
+}
+
+// ------------------------------------------------------------------ forward
+// Sums of x and x^2 of this workgroup's rows, by group, into put(group, sum, square).
+template <typename T, int PER, bool VEC, typename Put>
+__device__ __forceinline__ void sum_rows(const Args& a, const Rows& r, const Place& p, double* red, Put put) {
+  const int span = p.nx * PER, cg = a.C / a.G;
+  // red: [channels of a block, 2]: the rows' lanes are joined in LDS, channel block by channel block
+  for (int c0 = 0; c0 < a.C; c0 += span) {
+    const int c = c0 + p.tx * PER;
+    double s[PER], q[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] = q[i] = 0.0;
+    if (p.ty < p.ny && c < a.C)
+      for (int row = r.start + p.ty; row < r.end; row += p.ny) {
+        float v[PER];
+        load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          s[i] += (double)v[i];
+          q[i] = fma((double)v[i], (double)v[i], q[i]);
+        }
+      }
+    // [ny][channels of the block] in turn, summed by channel
+    for (int y = 0; y < p.ny; ++y) {
+      if (p.ty == y && c < a.C) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (c + i < a.C) {
+            double* at = red + 2 * (c0 + p.tx * PER + i);
+            at[0] = (y ? at[0] : 0.0) + s[i];
+            at[1] = (y ? at[1] : 0.0) + q[i];
+          }
+      }
+      __syncthreads();
+    }
+  }
+  group_sums<double>(
+      a.G, cg,
+      [&](int g, int i, double* t) {
+        t[0] = red[2 * (g * cg + i)];
+        t[1] = red[2 * (g * cg + i) + 1];
+      },
+      put);
+}
+
+template <typename T, int ACT, bool VEC>
+__device__ __forceinline__ void apply_rows(const Args& a, const Rows& r, const Place& p, const float* gstat) {
+  constexpr int PER = Vec<T>::kPer;
+  const int cg = a.C / a.G;
+  if (p.ty >= p.ny) return;
+  for (int c = p.tx * PER; c < a.C; c += p.nx * PER) {
+    float mean[PER], mul[PER], add[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int k = min(c + i, a.C - 1), g = k / cg;
+      mean[i] = gstat[2 * g];
+      mul[i] = gstat[2 * g + 1] * (a.w != nullptr ? a.w[k] : 1.f);
+      add[i] = a.b != nullptr ? a.b[k] : 0.f;
+    }
+    for (int row = r.start + p.ty; row < r.end; row += p.ny) {
+      float v[PER];
+      load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = act<ACT>(fmaf(v[i] - mean[i], mul[i], add[i]));
+      store<T, PER, VEC>((T*)a.y + (int64_t)row * a.C, c, a.C, v);
+    }
+  }
+}
+
+__device__ __forceinline__ void finish_stat(const Args& a, const Rows& r, int g, double s, double q, float* gstat) {
+  const double n = (double)r.length * (double)(a.C / a.G);
+  const double mean = s / n, var = q / n - mean * mean;
+  const double inv = 1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)a.eps);  // what is no number stays none
+  gstat[2 * g] = (float)mean;
+  gstat[2 * g + 1] = (float)inv;
+}
+
+template <typename T, int ACT, bool VEC>
+__global__ __launch_bounds__(kThreads) void fwd_whole_kernel(Args a) {
+  constexpr int PER = Vec<T>::kPer;
+  extern __shared__ __attribute__((aligned(16))) double red[];  // [C, 2], then [G, 2] floats
+  float* gstat = (float*)(red + 2 * a.C);
+  const Rows r = my_rows<true>(a);
+  const Place p = place(a.C, PER);
+  if (r.start >= r.end) return;
+  if (r.seq < 0) return zero_rows<T, PER, VEC>((T*)a.y, r, a.C, p);
+  sum_rows<T, PER, VEC>(a, r, p, red, [&](int g, double s, double q) { finish_stat(a, r, g, s, q, gstat); });
+  __syncthreads();
+  if (a.stat != nullptr)
+    for (int i = threadIdx.x; i < 2 * a.G; i += kThreads) a.stat[(int64_t)r.seq * 2 * a.G + i] = gstat[i];
+  apply_rows<T, ACT, VEC>(a, r, p, gstat);
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kThreads) void fwd_sums_kernel(Args a) {
+  constexpr int PER = Vec<T>::kPer;
+  extern __shared__ __attribute__((aligned(16))) double red[];
+  const Rows r = my_rows<false>(a);
+  if (r.start >= r.end || r.seq < 0) return;
+  double* to = a.part + (int64_t)blockIdx.x * 2 * a.G;
+  sum_rows<T, PER, VEC>(a, r, place(a.C, PER), red, [&](int g, double s, double q) {
+    to[2 * g] = s;
+    to[2 * g + 1] = q;
+  });
+}
+
+template <typename T, int ACT, bool VEC>
+__global__ __launch_bounds__(kThreads) void fwd_apply_kernel(Args a) {
+  constexpr int PER = Vec<T>::kPer;
+  extern __shared__ __attribute__((aligned(16))) double red[];
+  float* gstat = (float*)red;
+  const Rows r = my_rows<false>(a);
+  const Place p = place(a.C, PER);
+  if (r.start >= r.end) return;
+  if (r.seq < 0) return zero_rows<T, PER, VEC>((T*)a.y, r, a.C, p);
+  const double* from = a.part + (int64_t)r.first * 2 * a.G;
+  group_sums<double>(
+      a.G, r.chunks,
+      [&](int g, int i, double* t) {
+        t[0] = from[((int64_t)i * a.G + g) * 2];
+        t[1] = from[((int64_t)i * a.G + g) * 2 + 1];
+      },
+      [&](int g, double s, double q) { finish_stat(a, r, g, s, q, gstat); });
+  __syncthreads();
+  if (a.stat != nullptr && (int)blockIdx.x == r.first)
+    for (int i = threadIdx.x; i < 2 * a.G; i += kThreads) a.stat[(int64_t)r.seq * 2 * a.G + i] = gstat[i];
+  apply_rows<T, ACT, VEC>(a, r, p, gstat);
+}
+
+// ------------------------------------------------------------------ backward
+// Sums of dz and dz xh of this workgroup's rows: by channel into cpart (and red), by group through
+// put(group, sum of w dz, sum of w dz xh).
+template <typename T, int ACT, bool VEC, typename Put>
+__device__ __forceinline__ void grad_sums(const Args& a, const Rows& r, const Place& p, float* red, float* cpart,
+                                          Put put) {
+  constexpr int PER = Vec<T>::kPer;
+  const int span = p.nx * PER, cg = a.C / a.G;
+  const float* stat = a.stat + (int64_t)r.seq * 2 * a.G;
+  for (int c0 = 0; c0 < a.C; c0 += span) {
+    const int c = c0 + p.tx * PER;
+    float s[PER], q[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] = q[i] = 0.f;
+    if (p.ty < p.ny && c < a.C) {
+      float mean[PER], inv[PER], w[PER], b[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int k = min(c + i, a.C - 1), g = k / cg;
+        mean[i] = stat[2 * g];
+        inv[i] = stat[2 * g + 1];
+        w[i] = a.w != nullptr ? a.w[k] : 1.f;
+        b[i] = a.b != nullptr ? a.b[k] : 0.f;
+      }
+      for (int row = r.start + p.ty; row < r.end; row += p.ny) {
+        float v[PER], d[PER];
+        load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v);
+        load<T, PER, VEC>((const T*)a.dy + (int64_t)row * a.dy_row, c, a.C, d);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const float xh = (v[i] - mean[i]) * inv[i];
+          const float dz = d[i] * act_grad<ACT>(fmaf(xh, w[i], b[i]));
+          s[i] += dz;
+          q[i] = fmaf(dz, xh, q[i]);
+        }
+      }
+    }
+    for (int y = 0; y < p.ny; ++y) {
+      if (p.ty == y && c < a.C) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (c + i < a.C) {
+            float* at = red + 2 * (c + i);
+            at[0] = (y ? at[0] : 0.f) + s[i];
+            at[1] = (y ? at[1] : 0.f) + q[i];
+          }
+      }
+      __syncthreads();
+    }
+  }
+  for (int i = threadIdx.x; i < 2 * a.C; i += kThreads) cpart[i] = red[i];
+  group_sums<double>(
+      a.G, cg,
+      [&](int g, int i, double* t) {
+        const int k = g * cg + i;
+        const float w = a.w != nullptr ? a.w[k] : 1.f;
+        t[0] = (double)product(w, red[2 * k]);
+        t[1] = (double)product(w, red[2 * k + 1]);
+      },
+      put);
+}
+
+template <typename T, int ACT, bool VEC>
+__device__ __forceinline__ void grad_apply(const Args& a, const Rows& r, const Place& p, const float* gmean) {
+  constexpr int PER = Vec<T>::kPer;
+  const int cg = a.C / a.G;
+  const float* stat = a.stat + (int64_t)r.seq * 2 * a.G;
+  if (p.ty >= p.ny) return;
+  for (int c = p.tx * PER; c < a.C; c += p.nx * PER) {
+    float mean[PER], inv[PER], w[PER], b[PER], m1[PER], m2[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int k = min(c + i, a.C - 1), g = k / cg;
+      mean[i] = stat[2 * g];
+      inv[i] = stat[2 * g + 1];
+      w[i] = a.w != nullptr ? a.w[k] : 1.f;
+      b[i] = a.b != nullptr ? a.b[k] : 0.f;
+      m1[i] = gmean[2 * g];
+      m2[i] = gmean[2 * g + 1];
+    }
+    for (int row = r.start + p.ty; row < r.end; row += p.ny) {
+      float v[PER], d[PER];
+      load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v);
+      load<T, PER, VEC>((const T*)a.dy + (int64_t)row * a.dy_row, c, a.C, d);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const float xh = (v[i] - mean[i]) * inv[i];
+        const float dz = d[i] * act_grad<ACT>(fmaf(xh, w[i], b[i]));
+        v[i] = inv[i] * (product(w[i], dz) - m1[i] - xh * m2[i]);
+      }
+      store<T, PER, VEC>((T*)a.dx + (int64_t)row * a.C, c, a.C, v);
+    }
+  }
+}
+
+template <typename T, int ACT, bool VEC>
+__global__ __launch_bounds__(kThreads) void bwd_whole_kernel(Args a) {
+  constexpr int PER = Vec<T>::kPer;
+  extern __shared__ __attribute__((aligned(16))) double smem[];
+  float* red = (float*)smem;            // [C, 2]
+  float* gmean = red + 2 * a.C;         // [G, 2]
+  const Rows r = my_rows<true>(a);
+  const Place p = place(a.C, PER);
+  float* cpart = a.cpart + (int64_t)blockIdx.x * 2 * a.C;
+  if (r.start >= r.end || r.seq < 0) {
+    for (int i = threadIdx.x; i < 2 * a.C; i += kThreads) cpart[i] = 0.f;
+    return zero_rows<T, PER, VEC>((T*)a.dx, r, a.C, p);
+  }
+  const double n = (double)r.length * (double)(a.C / a.G);
+  grad_sums<T, ACT, VEC>(a, r, p, red, cpart, [&](int g, double s, double q) {
+    gmean[2 * g] = (float)(s / n);
+    gmean[2 * g + 1] = (float)(q / n);
+  });
+  __syncthreads();
+  grad_apply<T, ACT, VEC>(a, r, p, gmean);
+}
+
+template <typename T, int ACT, bool VEC>
+__global__ __launch_bounds__(kThreads) void bwd_sums_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(16))) double smem[];
+  const Rows r = my_rows<false>(a);
+  float* cpart = a.cpart + (int64_t)blockIdx.x * 2 * a.C;
+  if (r.start >= r.end || r.seq < 0) {
+    for (int i = threadIdx.x; i < 2 * a.C; i += kThreads) cpart[i] = 0.f;
+    return;
+  }
+  double* to = a.part + (int64_t)blockIdx.x * 2 * a.G;
+  grad_sums<T, ACT, VEC>(a, r, place(a.C, Vec<T>::kPer), (float*)smem, cpart, [&](int g, double s, double q) {
+    to[2 * g] = s;
+    to[2 * g + 1] = q;
+  });
+}
+
+template <typename T, int ACT, bool VEC>
+__global__ __launch_bounds__(kThreads) void bwd_apply_kernel(Args a) {
+  constexpr int PER = Vec<T>::kPer;
+  extern __shared__ __attribute__((aligned(16))) double smem[];
+  float* gmean = (float*)smem;
+  const Rows r = my_rows<false>(a);
+  const Place p = place(a.C, PER);
+  if (r.start >= r.end) return;
+  if (r.seq < 0) return zero_rows<T, PER, VEC>((T*)a.dx, r, a.C, p);
+  const double* from = a.part + (int64_t)r.first * 2 * a.G;
+  const double n = (double)r.length * (double)(a.C / a.G);
+  group_sums<double>(
+      a.G, r.chunks,
+      [&](int g, int i, double* t) {
+        t[0] = from[((int64_t)i * a.G + g) * 2];
+        t[1] = from[((int64_t)i * a.G + g) * 2 + 1];
+      },
+      [&](int g, double s, double q) {
+        gmean[2 * g] = (float)(s / n);
+        gmean[2 * g + 1] = (float)(q / n);
+      });
+  __syncthreads();
+  grad_apply<T, ACT, VEC>(a, r, p, gmean);
+}
+
+// dw, db: the chunks' sums of 16 channels a workgroup, 16 threads a channel, in 64 bits and in order
+__global__ __launch_bounds__(256) void bwd_param_kernel(Args a) {
+  __shared__ double sum[16][16][2];
+  const int ch = threadIdx.x & 15, part = threadIdx.x >> 4, c = blockIdx.x * 16 + ch;
+  double s = 0.0, q = 0.0;
+  if (c < a.C)
+    for (int i = part; i < a.chunks; i += 16) {
+      const float2 v = *reinterpret_cast<const float2*>(a.cpart + ((int64_t)i * a.C + c) * 2);
+      s += v.x;
+      q += v.y;
+    }
+  sum[part][ch][0] = s;
+  sum[part][ch][1] = q;
+  __syncthreads();
+  if (threadIdx.x < 16 && c < a.C) {
+    for (int i = 1; i < 16; ++i) {
+      s += sum[i][ch][0];
+      q += sum[i][ch][1];
+    }
+    a.db[c] = (float)s;
+    a.dw[c] = (float)q;
+  }
+}
+
+// ------------------------------------------------------------------ host
+// One workgroup a sequence where the average one is short enough that its second pass reads the
+// caches and there are enough of them, or so short that a second launch would cost more.
+static bool whole(const Args& a, int bytes) {
+  const int64_t avg = (int64_t)a.N / std::max(a.S, 1) * a.C * bytes;
+  return avg <= 64 * 1024;
+}
+
+static int chunk_rows(const Args& a, int per) {
+  const int ny = kThreads / std::min((a.C + per - 1) / per, kThreads);
+  // about four workgroups a compute unit, at least 8 rows a thread
+  const int64_t rows = std::max<int64_t>(((int64_t)a.N + 4 * num_cus() - 1) / (4 * num_cus()), 8 * ny);
+  return (int)std::min<int64_t>(rows, 1 << 20);
+}
+
+// above 64 KB of LDS only many thousand channels get
+template <typename K>
+static void launch(K* kern, int blocks, size_t lds, hipStream_t st, const Args& a) {
+  if (lds > 65536) (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  kern<<<dim3(blocks), kThreads, lds, st>>>(a);
+}
+
+template <typename T, int ACT, bool VEC>
+static void forward(Args a, hipStream_t st, const at::TensorOptions& opt) {
+  const size_t lds = a.C * 16 + a.G * 8;
+  if (whole(a, sizeof(T))) {
+    launch(&fwd_whole_kernel<T, ACT, VEC>, a.S + 2, lds, st, a);
+    return;
+  }
+  a.chunk = chunk_rows(a, Vec<T>::kPer);
+  a.chunks = (int)tile_count(a.N, a.S, a.chunk);
+  at::Tensor part = at::empty({(int64_t)a.chunks * 2 * a.G}, opt.dtype(at::kDouble));
+  a.part = part.data_ptr<double>();
+  launch(&fwd_sums_kernel<T, VEC>, a.chunks, a.C * 16, st, a);
+  launch(&fwd_apply_kernel<T, ACT, VEC>, a.chunks, a.G * 8, st, a);
+}
+
+template <typename T, int ACT, bool VEC>
+static void backward(Args a, hipStream_t st, const at::TensorOptions& opt) {
+  const size_t lds = a.C * 8 + a.G * 8;
+  at::Tensor part, cpart;
+  if (whole(a, 2 * sizeof(T))) {
+    a.chunks = a.S + 2;
+    cpart = at::empty({(int64_t)a.chunks * 2 * a.C}, opt.dtype(at::kFloat));
+    a.cpart = cpart.data_ptr<float>();
+    launch(&bwd_whole_kernel<T, ACT, VEC>, a.chunks, lds, st, a);
+  } else {
+    a.chunk = chunk_rows(a, Vec<T>::kPer);
+    a.chunks = (int)tile_count(a.N, a.S, a.chunk);
+    part = at::empty({(int64_t)a.chunks * 2 * a.G}, opt.dtype(at::kDouble));
+    cpart = at::empty({(int64_t)a.chunks * 2 * a.C}, opt.dtype(at::kFloat));
+    a.part = part.data_ptr<double>();
+    a.cpart = cpart.data_ptr<float>();
+    launch(&bwd_sums_kernel<T, ACT, VEC>, a.chunks, lds, st, a);
+    launch(&bwd_apply_kernel<T, ACT, VEC>, a.chunks, a.G * 8, st, a);
+  }
+  bwd_param_kernel<<<dim3(ceil_div(a.C, 16)), 256, 0, st>>>(a);
+}
+
+template <typename T, bool VEC>
+static void by_act(const Args& a, int act, bool back, hipStream_t st, const at::TensorOptions& opt) {
+  if (act == kNone) back ? backward<T, kNone, VEC>(a, st, opt) : forward<T, kNone, VEC>(a, st, opt);
+  else if (act == kRelu) back ? backward<T, kRelu, VEC>(a, st, opt) : forward<T, kRelu, VEC>(a, st, opt);
+  else back ? backward<T, kSilu, VEC>(a, st, opt) : forward<T, kSilu, VEC>(a, st, opt);
+}
+
+static void by_type(const Args& a, at::ScalarType t, bool vec, int act, bool back, hipStream_t st,
+                    const at::TensorOptions& opt) {
+  if (t == at::kFloat) vec ? by_act<float, true>(a, act, back, st, opt) : by_act<float, false>(a, act, back, st, opt);
+  else if (t == at::kBFloat16)
+    vec ? by_act<__bf16, true>(a, act, back, st, opt) : by_act<__bf16, false>(a, act, back, st, opt);
+  else vec ? by_act<_Float16, true>(a, act, back, st, opt) : by_act<_Float16, false>(a, act, back, st, opt);
+}
+
+typedef c10::optional<at::Tensor> OptTensor;
+
+static bool vec16(const at::Tensor& t) {
+  const int64_t per = 16 / t.element_size();
+  return t.size(1) % per == 0 && t.stride(0) % per == 0 && ((uintptr_t)t.data_ptr() & 15) == 0;
+}
+
+static at::Tensor rows(const at::Tensor& t) { return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous(); }
+
+static Args fill(const at::Tensor& x, const OptTensor& w, const OptTensor& b, const OptTensor& ptr, int64_t seqs,
+                 int64_t groups, double eps) {
+  const auto t = x.scalar_type();
+  HY_CHECK(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "group_norm: x must be fp32, bf16 or fp16");
+  HY_CHECK(x.dim() == 2 && x.size(0) < INT_MAX / 2 && x.size(1) >= 1 && x.size(1) <= 4096, "group_norm: x shape");
+  HY_CHECK(groups >= 1 && x.size(1) % groups == 0, "group_norm: groups must divide the channels");
+  Args a = {};
+  a.x = x.data_ptr();
+  a.x_row = x.stride(0);
+  a.N = (int)x.size(0);
+  a.C = (int)x.size(1);
+  a.G = (int)groups;
+  a.eps = (float)eps;
+  for (const auto* p : {&w, &b})
+    HY_CHECK(!p->has_value() || ((*p)->device() == x.device() && (*p)->scalar_type() == at::kFloat &&
+                                 (*p)->is_contiguous() && (*p)->numel() == x.size(1)),
+             "group_norm: weight and bias must be contiguous fp32 [channels] on x's device");
+  a.w = w.has_value() ? w->data_ptr<float>() : nullptr;
+  a.b = b.has_value() ? b->data_ptr<float>() : nullptr;
+  if (ptr.has_value()) {
+    HY_CHECK(ptr->device() == x.device() && ptr->scalar_type() == at::kInt && ptr->is_contiguous() &&
+                 ptr->dim() == 1 && ptr->numel() >= 1,
+             "group_norm: ptr must be contiguous int32 on x's device");
+    a.ptr = ptr->data_ptr<int>();
+    a.S = (int)ptr->numel() - 1;
+  } else {
+    HY_CHECK(seqs >= 0 && seqs < INT_MAX / 4 && (seqs == 0 || x.size(0) % seqs == 0), "group_norm: samples");
+    a.S = (int)seqs;
+    a.uniform = seqs ? x.size(0) / seqs : 0;
+  }
+  return a;
+}
+
+std::tuple<at::Tensor, at::Tensor> group_norm_fwd(const at::Tensor& x_, const OptTensor& w, const OptTensor& b,
+                                                  const OptTensor& ptr, int64_t seqs, int64_t groups, double eps,
+                                                  int64_t act, bool save) {
+  HY_CHECK_CUDA(x_);
+  c10::DeviceGuard guard(x_.device());
+  const at::Tensor x = rows(x_);
+  Args a = fill(x, w, b, ptr, seqs, groups, eps);
+  at::Tensor y = at::empty({x.size(0), x.size(1)}, x.options());
+  at::Tensor stat = at::empty({save ? a.S : 0, a.G, 2}, x.options().dtype(at::kFloat));
+  if (a.N == 0) return {y, stat};
+  a.y = y.data_ptr();
+  a.stat = save ? stat.data_ptr<float>() : nullptr;
+  by_type(a, x.scalar_type(), vec16(x), (int)act, false, stream(), x.options());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return {y, stat};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> group_norm_bwd(const at::Tensor& dy_, const at::Tensor& x_,
+                                                              const at::Tensor& stat, const OptTensor& w,
+                                                              const OptTensor& b, const OptTensor& ptr, int64_t seqs,
+                                                              int64_t groups, double eps, int64_t act) {
+  HY_CHECK_CUDA(x_);
+  c10::DeviceGuard guard(x_.device());
+  const at::Tensor x = rows(x_);
+  HY_CHECK(dy_.sizes() == x.sizes() && dy_.scalar_type() == x.scalar_type() && dy_.device() == x.device(),
+           "group_norm: the output's gradient must be like the output");
+  const at::Tensor dy = rows(dy_);
+  Args a = fill(x, w, b, ptr, seqs, groups, eps);
+  HY_CHECK(stat.is_contiguous() && stat.scalar_type() == at::kFloat && stat.numel() == (int64_t)a.S * a.G * 2,
+           "group_norm: saved statistics");
+  const auto f32 = x.options().dtype(at::kFloat);
+  at::Tensor dx = at::empty({x.size(0), x.size(1)}, x.options());
+  at::Tensor dw = at::empty({x.size(1)}, f32), db = at::empty({x.size(1)}, f32);
+  a.dy = dy.data_ptr();
+  a.dy_row = dy.stride(0);
+  a.dx = dx.data_ptr();
+  a.dw = dw.data_ptr<float>();
+  a.db = db.data_ptr<float>();
+  a.stat = stat.data_ptr<float>();
+  by_type(a, x.scalar_type(), vec16(x) && vec16(dy), (int)act, true, stream(), x.options());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return {dx, dw, db};
+}
+
+}  // namespace gn
+}  // namespace hy
+
+TORCH_LIBRARY_FRAGMENT(hydra, m) {
+  m.def(
+      "group_norm_fwd(Tensor x, Tensor? weight, Tensor? bias, Tensor? ptr, int seqs, int groups, float eps, int act, "
+      "bool save) -> (Tensor, Tensor)");
+  m.def(
+      "group_norm_bwd(Tensor dy, Tensor x, Tensor stat, Tensor? weight, Tensor? bias, Tensor? ptr, int seqs, "
+      "int groups, float eps, int act) -> (Tensor, Tensor, Tensor)");
+}
+TORCH_LIBRARY_IMPL(hydra, CUDA, m) {
+  m.impl("group_norm_fwd", hy::gn::group_norm_fwd);
+  m.impl("group_norm_bwd", hy::gn::group_norm_bwd);
+}

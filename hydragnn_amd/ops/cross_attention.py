@@ -1,0 +1,257 @@
+"""Multi-head attention of one ragged batch's rows on another's, with an optional learned
+relative position bias.
+
+    o_i = sum_j softmax_j(scale q_i . k_j + table[h, bucket(q_pos_i, k_pos_j)]) v_j
+
+Row i of sequence s sees the keys of sequence s that ``key_mask`` keeps: ``q_ptr`` and ``k_ptr``
+are the CSR row pointers of the two sides, whose lengths are independent (read-out queries on a
+graph's nodes, a decoder's rows on an encoder's, one token on a long state).  Next to
+``ops.attention.segment_attention`` (packed fp32 self attention over segments).
+
+GPU: ``csrc/cross_attn_*.hip``.  CPU, and the composite (double-backward) mode: plain torch.
+"""
+import functools
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _native
+from . import pna as _mode
+
+MAX_WIDTH = 128  # of a head
+MAX_BUCKETS = 64
+MAX_DISTANCE = 2048
+_GPU_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+@functools.lru_cache(maxsize=256)
+def _rule(side, far):
+    """(near, thresholds): distances below ``near = side // 2`` have a bucket each, and bucket
+    near + j begins at the first whole n with (n / near) ** (side - near) >= (far / near) ** j.
+    Whole numbers only: no rounding moves a border."""
+    near = side // 2
+    steps = side - near
+    thr = []
+    for j in range(1, steps):
+        lo, hi = near, far
+        while lo < hi:
+            n = (lo + hi) // 2
+            if n ** steps * near ** j >= far ** j * near ** steps:
+                hi = n
+            else:
+                lo = n + 1
+        thr.append(lo)
+    return near, tuple(thr)
+
+
+class RelativeBuckets:
+    """The bucket of a pair of positions.
+
+    A whole distance n has bucket n below ``near``, half of the buckets; from there to
+    ``max_distance`` the rest are spread over log n, and all farther pairs share the last.
+
+    * ``unit=None``: positions are whole numbers (int32 [rows], the order of a sequence), n is
+      |k_pos - q_pos|.  ``bidirectional``: keys behind the query have the second half of the
+      ``num_buckets``; otherwise they all count as distance 0.
+    * ``unit=u``: positions are points (fp32 [rows, 3]), n is floor(distance / u), exact to the
+      border (64-bit arithmetic where 32 bits leave a doubt).  A distance that is not a number
+      counts as far.
+
+    >>> RelativeBuckets(32, 128)             # orders, both directions
+    >>> RelativeBuckets(32, 64, unit=0.25)   # distances: steps of 0.25 up to 4, then wider, far from 16 on
+    """
+
+    def __init__(self, num_buckets=32, max_distance=128, bidirectional=True, unit=None):
+        two_sided = bool(bidirectional) and unit is None
+        if not isinstance(num_buckets, int) or not 2 <= num_buckets <= MAX_BUCKETS:
+            raise ValueError(f"num_buckets must be a whole number from 2 to {MAX_BUCKETS}, got {num_buckets!r}")
+        if two_sided and (num_buckets % 2 or num_buckets < 4):
+            raise ValueError(f"bidirectional buckets need an even number of at least 4, got {num_buckets}")
+        side = num_buckets // 2 if two_sided else num_buckets
+        if not isinstance(max_distance, int) or not side // 2 < max_distance <= MAX_DISTANCE:
+            raise ValueError(f"max_distance must be a whole number above {side // 2}, the exact buckets, "
+                             f"and at most {MAX_DISTANCE}, got {max_distance!r}")
+        if unit is not None and not 1e-12 <= float(unit) <= 1e12:
+            raise ValueError(f"unit must lie between 1e-12 and 1e12, got {unit!r}")
+        self.num_buckets, self.max_distance, self.bidirectional = num_buckets, max_distance, two_sided
+        self.unit = None if unit is None else float(unit)
+        self.side = side
+        self.near, self.thresholds = _rule(side, max_distance)
+        self.rule = [int(two_sided), side, self.near, max_distance, *self.thresholds]
+
+    def __repr__(self):
+        return (f"RelativeBuckets({self.num_buckets}, {self.max_distance}, bidirectional={self.bidirectional}, "
+                f"unit={self.unit})")
+
+    def buckets(self, q_pos, k_pos):
+        """Bucket numbers [..., Lq, Lk] of positions [..., Lq(, 3)] and [..., Lk(, 3)] (plain torch)."""
+        first = 0
+        if self.unit is not None:
+            d = k_pos.double().unsqueeze(-3) - q_pos.double().unsqueeze(-2)
+            d = torch.sqrt(d[..., 0] * d[..., 0] + d[..., 1] * d[..., 1] + d[..., 2] * d[..., 2]) / self.unit
+            n = torch.where(d < self.max_distance, d, torch.full_like(d, self.max_distance)).long()
+        else:
+            rel = k_pos.long().unsqueeze(-2) - q_pos.long().unsqueeze(-1)
+            if self.bidirectional:
+                first, n = (rel > 0).long() * self.side, rel.abs()
+            else:
+                n = (-rel).clamp(min=0)
+        thr = torch.tensor(self.thresholds, dtype=torch.long, device=n.device)
+        return first + torch.where(n < self.near, n, self.near + torch.bucketize(n, thr, right=True))
+
+
+def _check(q, k, v, q_ptr, k_ptr, key_mask, table, buckets, q_pos, k_pos):
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("cross_attention: q, k and v are [rows, heads, width]")
+    if k.shape != v.shape:
+        raise ValueError(f"cross_attention: k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError(f"cross_attention: q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}")
+    if q.dtype not in _GPU_TYPES and not (q.dtype == torch.float64 and not q.is_cuda):
+        raise ValueError(f"cross_attention: {q.dtype} is not supported")
+    H, D, Hk = q.shape[1], q.shape[2], k.shape[1]
+    if k.shape[2] != D or not 1 <= D <= MAX_WIDTH:
+        raise ValueError(f"cross_attention: q and k need one head width of 1 to {MAX_WIDTH}, got {D} and {k.shape[2]}")
+    if Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"cross_attention: {H} query heads are no multiple of {Hk} key heads")
+    dev = q.device
+    for name, t in (("k", k), ("v", v), ("q_ptr", q_ptr), ("k_ptr", k_ptr), ("key_mask", key_mask), ("table", table),
+                    ("q_pos", q_pos), ("k_pos", k_pos)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"cross_attention: {name} is on {t.device}, q on {dev}")
+    if q_ptr.dtype != torch.int32 or k_ptr.dtype != torch.int32 or q_ptr.dim() != 1 or q_ptr.shape != k_ptr.shape \
+            or q_ptr.shape[0] < 1:
+        raise ValueError("cross_attention: q_ptr and k_ptr are int32 [sequences + 1]")
+    if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.shape != k.shape[:1]):
+        raise ValueError("cross_attention: key_mask is bool [key rows]")
+    if (table is None) != (buckets is None):
+        raise ValueError("cross_attention: table and buckets go together")
+    if table is not None:
+        if table.dtype not in (torch.float32, q.dtype) or table.shape != (H, buckets.num_buckets):
+            raise ValueError(f"cross_attention: table is float32 (or q's type) [{H}, {buckets.num_buckets}], got "
+                             f"{table.dtype} {tuple(table.shape)}")
+        want, tail = (torch.int32, ()) if buckets.unit is None else (torch.float32, (3,))
+        for name, p, rows in (("q_pos", q_pos, q.shape[0]), ("k_pos", k_pos, k.shape[0])):
+            if p is None or p.dtype != want or p.shape != (rows,) + tail:
+                raise ValueError(f"cross_attention: {name} must be {want} {[rows, *tail]}"
+                                 + (", got none" if p is None else f", got {p.dtype} {list(p.shape)}"))
+    elif q_pos is not None or k_pos is not None:
+        raise ValueError("cross_attention: positions without a table")
+
+
+class _CrossAttn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_ptr, k_ptr, key_mask, scale, table, q_pos, k_pos, rule, unit):
+        out, rest, lse = _native.ops().cross_attn_fwd(q, k, v, q_ptr, k_ptr, key_mask, scale, table, q_pos, k_pos,
+                                                      rule, unit, True)
+        ctx.save_for_backward(q, k, v, out, rest, lse, q_ptr, k_ptr, key_mask, table, q_pos, k_pos)
+        ctx.cfg = scale, rule, unit
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        q, k, v, out, rest, lse, q_ptr, k_ptr, key_mask, table, q_pos, k_pos = ctx.saved_tensors
+        scale, rule, unit = ctx.cfg
+        dq, dk, dv, dt = _native.ops().cross_attn_bwd(d_out, q, k, v, out, rest, lse, q_ptr, k_ptr, key_mask, scale,
+                                                      table, q_pos, k_pos, rule, unit)
+        return dq, dk, dv, None, None, None, None, None if table is None else dt, None, None, None, None
+
+
+def cross_attention(q, k, v, q_ptr, k_ptr, scale=None, key_mask=None, table=None, buckets=None, q_pos=None,
+                    k_pos=None):
+    """Attention of ``q`` [Nq, H, D] on ``k``, ``v`` [Nk, Hk, D] -> [Nq, H, D].
+
+    * ``q_ptr``, ``k_ptr``: int32 [S + 1], ascending from 0; sequence s has the query rows
+      q_ptr[s]..q_ptr[s + 1] and the key rows k_ptr[s]..k_ptr[s + 1], either of any number, 0 too.
+      Rows behind the last sequence (the padding of a statically shaped batch) take no part: their
+      outputs and gradients are zeros, whatever they hold.
+    * query head h uses key head h // (H / Hk); H a multiple of Hk.
+    * types: float32, bfloat16, float16 (float64 on the CPU); statistics and sums are held in 32
+      bits.  Rows and heads may be strided (views of a packed projection are read in place).
+    * ``scale``: 1 / sqrt(D) if not given.
+    * ``key_mask``: bool [Nk]; a key without it takes no part, whatever it holds.  A row that has
+      no key gives zeros and passes no gradient on.
+    * ``table`` [H, buckets.num_buckets], ``buckets`` (:class:`RelativeBuckets`), ``q_pos``,
+      ``k_pos``: the relative position bias; the table's gradient is float32 sums over all pairs.
+
+    Pointers that do not ascend give unspecified outputs on the GPU (nothing outside the tensors
+    is read or written) and raise on the CPU.  Differentiable once in q, k, v and table on the GPU.
+    """
+    _check(q, k, v, q_ptr, k_ptr, key_mask, table, buckets, q_pos, k_pos)
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    if not q.is_cuda or not _mode.fused("attn"):
+        return cross_attention_reference(q, k, v, q_ptr, k_ptr, scale, key_mask, table, buckets, q_pos, k_pos)
+    rule, unit = ([], 0.0) if buckets is None else (buckets.rule, buckets.unit or 0.0)
+    if table is not None:
+        table, q_pos, k_pos = table.float().contiguous(), q_pos.contiguous(), k_pos.contiguous()
+    if key_mask is not None:
+        key_mask = key_mask.contiguous()
+    q_ptr, k_ptr = q_ptr.contiguous(), k_ptr.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (table is not None and table.requires_grad)):
+        return _CrossAttn.apply(q, k, v, q_ptr, k_ptr, key_mask, scale, table, q_pos, k_pos, rule, unit)
+    return _native.ops().cross_attn_fwd(q, k, v, q_ptr, k_ptr, key_mask, scale, table, q_pos, k_pos, rule, unit,
+                                        False)[0]
+
+
+def _attend(q, k, v, scale, bias):
+    """[Lq, H, D] on [Lk, Hk, D], every key taking part (Lk >= 1)."""
+    g = q.shape[1] // k.shape[1]
+    if g > 1:
+        k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+    s = torch.matmul(q.transpose(0, 1), k.permute(1, 2, 0).contiguous()) * scale
+    if bias is not None:
+        s = s + bias
+    return torch.matmul(torch.softmax(s, -1), v.transpose(0, 1).contiguous()).transpose(0, 1)
+
+
+def cross_attention_reference(q, k, v, q_ptr, k_ptr, scale, key_mask=None, table=None, buckets=None, q_pos=None,
+                              k_pos=None):
+    """Plain torch, sequence by sequence: the CPU path, the oracle of the kernels' tests, and the
+    composite mode (differentiable to any order; while a graph is captured, as one masked score
+    matrix without a look at the pointers)."""
+    wide = q.dtype if q.dtype == torch.float64 else torch.float32
+    qf, kf, vf = q.to(wide), k.to(wide), v.to(wide)
+    tab = None if table is None else table.to(wide)
+    if q.is_cuda and torch.cuda.is_current_stream_capturing():
+        return _masked_reference(qf, kf, vf, q_ptr, k_ptr, scale, key_mask, tab, buckets, q_pos, k_pos).to(q.dtype)
+    qp, kp = q_ptr.tolist(), k_ptr.tolist()
+    for p, rows, name in ((qp, q.shape[0], "q_ptr"), (kp, k.shape[0], "k_ptr")):
+        if p[0] != 0 or p[-1] > rows or any(a > b for a, b in zip(p, p[1:])):
+            raise ValueError(f"cross_attention: {name} must ascend from 0 to at most {rows}")
+    parts = []
+    for a, b, c, d in zip(qp, qp[1:], kp, kp[1:]):
+        kk, vv, pos = kf[c:d], vf[c:d], None if k_pos is None else k_pos[c:d]
+        if key_mask is not None:
+            keep = key_mask[c:d].nonzero().view(-1)
+            kk, vv, pos = kk[keep], vv[keep], None if pos is None else pos[keep]
+        if a == b or kk.shape[0] == 0:
+            parts.append(qf.new_zeros((b - a,) + tuple(q.shape[1:])))
+            continue
+        bias = None if tab is None else tab[:, buckets.buckets(q_pos[a:b], pos)]
+        parts.append(_attend(qf[a:b], kk, vv, scale, bias))
+    parts.append(qf.new_zeros((q.shape[0] - qp[-1],) + tuple(q.shape[1:])))
+    return torch.cat(parts).to(q.dtype)
+
+
+def _masked_reference(q, k, v, q_ptr, k_ptr, scale, key_mask, table, buckets, q_pos, k_pos):
+    def seq(ptr, rows):  # sequence of each row; -1: none
+        r = torch.arange(rows, device=ptr.device, dtype=ptr.dtype)
+        s = torch.searchsorted(ptr, r, right=True) - 1
+        return torch.where(s < ptr.numel() - 1, s, torch.full_like(s, -1))
+
+    qs, ks = seq(q_ptr, q.shape[0]), seq(k_ptr, k.shape[0])
+    takes = ks >= 0 if key_mask is None else (ks >= 0) & key_mask
+    k, v = (torch.where(takes.view(-1, 1, 1), t, torch.zeros_like(t)) for t in (k, v))
+    q = torch.where((qs >= 0).view(-1, 1, 1), q, torch.zeros_like(q))
+    pair = (qs.view(-1, 1) == ks.view(1, -1)) & takes.view(1, -1)
+    g = q.shape[1] // k.shape[1]
+    if g > 1:
+        k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+    s = torch.matmul(q.transpose(0, 1), k.permute(1, 2, 0).contiguous()) * scale
+    if table is not None:
+        s = s + table[:, buckets.buckets(q_pos, k_pos)]
+    p = torch.softmax(s.masked_fill(~pair, torch.finfo(s.dtype).min), -1) * pair
+    return torch.matmul(p, v.transpose(0, 1).contiguous()).transpose(0, 1)

@@ -7,9 +7,13 @@ exact reference statistics.
 
 GPU training mode runs the two-pass HIP kernels of ``csrc/batchnorm.hip``
 (2 launches forward, 2 backward); CPU / eval / composite mode use torch ops.
+
+``group_norm``: statistics of each graph's own rows by groups of channels, with an activation
+(``csrc/group_norm.hip``).
 """
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .. import _native
 from . import pna as _mode
@@ -141,3 +145,120 @@ def norm_add(a, bn, num_valid=None, residual=None, p=0.0, relu=False, zero_pad=F
         rows = torch.arange(h.shape[0], device=h.device).view(-1, 1)
         h = h * (rows < num_valid).to(h.dtype)
     return h
+
+
+# ---------------------------------------------------------------------- group norm
+_ACTS = {"none": 0, "relu": 1, "silu": 2}
+GROUP_NORM_MAX_CHANNELS = 4096
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, ptr, seqs, groups, eps, act):
+        y, stat = _native.ops().group_norm_fwd(x, weight, bias, ptr, seqs, groups, eps, act, True)
+        ctx.save_for_backward(x, stat, weight, bias, ptr)
+        ctx.cfg = seqs, groups, eps, act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, stat, weight, bias, ptr = ctx.saved_tensors
+        dx, dw, db = _native.ops().group_norm_bwd(dy, x, stat, weight, bias, ptr, *ctx.cfg)
+        return dx, dw if weight is not None else None, db if bias is not None else None, None, None, None, None, None
+
+
+def _check_group_norm(x, groups, weight, bias, ptr, act):
+    if x.dim() < 2:
+        raise ValueError("group_norm: x is [rows, channels] or [samples, ..., channels]")
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16) and not (x.dtype == torch.float64
+                                                                              and not x.is_cuda):
+        raise ValueError(f"group_norm: {x.dtype} is not supported")
+    C = x.shape[-1]
+    if not 1 <= C <= GROUP_NORM_MAX_CHANNELS:
+        raise ValueError(f"group_norm: 1 to {GROUP_NORM_MAX_CHANNELS} channels, got {C}")
+    if not isinstance(groups, int) or groups < 1 or C % groups:
+        raise ValueError(f"group_norm: {groups!r} groups do not divide {C} channels")
+    if act not in _ACTS:
+        raise ValueError(f"group_norm: act is one of {sorted(_ACTS)}, got {act!r}")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.shape != (C,) or p.device != x.device or p.dtype not in (torch.float32, x.dtype)):
+            raise ValueError(f"group_norm: {name} is float32 (or x's type) [{C}] on {x.device}, got {p.dtype} "
+                             f"{tuple(p.shape)} on {p.device}")
+    if ptr is not None:
+        if x.dim() != 2:
+            raise ValueError("group_norm: with ptr, x is [rows, channels]")
+        if ptr.dtype != torch.int32 or ptr.dim() != 1 or ptr.shape[0] < 1 or ptr.device != x.device:
+            raise ValueError(f"group_norm: ptr is int32 [sequences + 1] on {x.device}")
+
+
+def group_norm(x, groups, weight=None, bias=None, ptr=None, eps=1e-5, act="none"):
+    """``act((x - mean) / sqrt(var + eps) * weight + bias)``, channels last.
+
+    Mean and (biased) variance go over the rows of one sequence and the ``C / groups`` channels of
+    one group, so a graph's features do not depend on the rest of its batch (``batch_norm``'s do).
+
+    * ``ptr`` int32 [S + 1]: CSR pointers of ``x`` [rows, C], ascending from 0, as a batch's graphs
+      lie behind each other; empty sequences are allowed.  Rows behind the last one (padding) give
+      zeros and pass no gradient on, whatever they hold.
+    * without ``ptr``: ``x`` [samples, ..., C], each sample by itself (an image [B, H, W, C]).
+    * types: float32, bfloat16, float16 (float64 on the CPU); ``weight`` and ``bias`` float32 or x's
+      type, [C], or None.  Rows may be strided.  ``act``: "none", "relu" or "silu".
+
+    Statistics are summed in 64 bits.  Differentiable once in x, weight and bias on the GPU.
+    """
+    _check_group_norm(x, groups, weight, bias, ptr, act)
+    if not x.is_cuda or not _mode.fused("norm"):
+        return group_norm_reference(x, groups, weight, bias, ptr, eps, act)
+    shape = x.shape
+    seqs = 0
+    if ptr is None:
+        seqs = shape[0]
+        x = x.reshape(-1, shape[-1])
+    else:
+        ptr = ptr.contiguous()
+    w, b = (None if p is None else p.float().contiguous() for p in (weight, bias))
+    if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)
+                                    or (b is not None and b.requires_grad)):
+        y = _GroupNorm.apply(x, w, b, ptr, seqs, groups, float(eps), _ACTS[act])
+    else:
+        y = _native.ops().group_norm_fwd(x, w, b, ptr, seqs, groups, float(eps), _ACTS[act], False)[0]
+    return y if y.shape == shape else y.view(shape)
+
+
+def group_norm_reference(x, groups, weight, bias, ptr, eps=1e-5, act="none"):
+    """Plain torch (the CPU path, the oracle of the kernels' tests, the composite mode), without a
+    look at the pointers on the host: sums by sequence through an index."""
+    shape, dtype = x.shape, x.dtype
+    wide = dtype if dtype == torch.float64 else torch.float32
+    C = shape[-1]
+    rows = x.reshape(-1, C)
+    N = rows.shape[0]
+    if ptr is None:
+        S = shape[0]
+        sid = torch.arange(S, device=x.device).repeat_interleave(N // S if S else 0)
+        there = None
+    else:
+        if not ptr.is_cuda:
+            p = ptr.tolist()
+            if p[0] != 0 or p[-1] > N or any(a > b for a, b in zip(p, p[1:])):
+                raise ValueError(f"group_norm: ptr must ascend from 0 to at most {N}")
+        S = ptr.numel() - 1
+        sid = torch.searchsorted(ptr, torch.arange(N, device=x.device, dtype=torch.int32), right=True) - 1
+        there = (sid < S).view(-1, 1)
+        rows = torch.where(there, rows, torch.zeros_like(rows))
+    v = rows.to(torch.float64).view(N, groups, C // groups)
+    here = torch.ones(N, dtype=torch.float64, device=x.device)
+    count = here.new_zeros(S + 1).index_add(0, sid, here).clamp(min=1).view(-1, 1) * (C // groups)
+    mean = v.new_zeros(S + 1, groups).index_add(0, sid, v.sum(-1)) / count
+    xc = v - mean[sid].unsqueeze(-1)
+    var = v.new_zeros(S + 1, groups).index_add(0, sid, (xc * xc).sum(-1)) / count
+    z = (xc * torch.rsqrt(var + eps)[sid].unsqueeze(-1)).view(N, C).to(wide)
+    if weight is not None:
+        z = z * weight.to(wide)
+    if bias is not None:
+        z = z + bias.to(wide)
+    z = {"none": lambda t: t, "relu": torch.relu, "silu": F.silu}[act](z)
+    if there is not None:
+        z = torch.where(there, z, torch.zeros_like(z))
+    return z.to(dtype).view(shape)
