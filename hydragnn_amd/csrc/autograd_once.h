@@ -1,0 +1,27 @@
+// Autograd functions in C++ whose gradients have no gradient of their own.
+#pragma once
+
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+namespace hy {
+
+// A backward's results.  Where they are asked for with a graph (create_graph), a second derivative
+// through them raises `what` instead of leaving its term out.
+inline torch::autograd::variable_list once(torch::autograd::variable_list res, const char* what) {
+  if (!at::GradMode::is_enabled()) return res;
+  std::vector<size_t> at;
+  torch::autograd::variable_list in;
+  for (size_t i = 0; i < res.size(); ++i)
+    if (res[i].defined()) {
+      at.push_back(i);
+      in.push_back(res[i].detach().set_requires_grad(true));
+    }
+  if (in.empty()) return res;
+  auto node = std::make_shared<torch::autograd::DelayedError>(what, in.size());
+  auto out = (*node)(std::move(in));
+  for (size_t i = 0; i < at.size(); ++i) res[at[i]] = out[i];
+  return res;
+}
+
+}  // namespace hy

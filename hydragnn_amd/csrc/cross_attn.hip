@@ -1,6 +1,7 @@
 // Ragged cross attention: the operators' entries (arguments, outputs, workspaces).
 #include <c10/core/DeviceGuard.h>
 
+#include "autograd_once.h"
 #include "cross_attn.h"
 
 namespace hy {
@@ -96,7 +97,7 @@ static int fill(Args& a, const at::Tensor& q, const at::Tensor& k, const at::Ten
   return bias;
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_fwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
+static std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_fwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
                                                   const at::Tensor& q_ptr, const at::Tensor& k_ptr,
                                                   const OptTensor& mask, double scale, const OptTensor& table,
                                                   const OptTensor& q_pos, const OptTensor& k_pos, at::IntArrayRef rule,
@@ -118,7 +119,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_fwd(const at::Tensor& 
   return {out, rest, lse};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd(
+static std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd(
     const at::Tensor& d_out, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& out,
     const at::Tensor& rest, const at::Tensor& lse, const at::Tensor& q_ptr, const at::Tensor& k_ptr, const OptTensor& mask, double scale,
     const OptTensor& table, const OptTensor& q_pos, const OptTensor& k_pos, at::IntArrayRef rule, double unit) {
@@ -160,19 +161,69 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd(
   return {dq, dk, dv, dtable};
 }
 
+// ------------------------------------------------------------------ autograd
+// In C++, because a small training step is bound by the calls around its kernels: the pair of calls
+// of a step costs about a third of what a Python autograd function's costs.
+struct CrossAttn : public torch::autograd::Function<CrossAttn> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
+                            const at::Tensor& v, const at::Tensor& q_ptr, const at::Tensor& k_ptr,
+                            const OptTensor& mask, double scale, const OptTensor& table, const OptTensor& q_pos,
+                            const OptTensor& k_pos, const std::vector<int64_t>& rule, double unit) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, rest, lse] =
+        cross_attn_fwd(q, k, v, q_ptr, k_ptr, mask, scale, table, q_pos, k_pos, rule, unit, true);
+    auto some = [](const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); };
+    ctx->save_for_backward({q, k, v, out, rest, lse, q_ptr, k_ptr, some(mask), some(table), some(q_pos), some(k_pos)});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["rule"] = rule;
+    ctx->saved_data["unit"] = unit;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    auto some = [](const at::Tensor& x) { return x.defined() ? OptTensor(x) : OptTensor(); };
+    const auto rule = ctx->saved_data["rule"].toIntVector();
+    torch::autograd::variable_list res(12);
+    if (!grads[0].defined()) return res;
+    {
+      at::AutoGradMode off(false);
+      auto [dq, dk, dv, dt] = cross_attn_bwd(grads[0], t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], some(t[8]),
+                                             ctx->saved_data["scale"].toDouble(), some(t[9]), some(t[10]), some(t[11]),
+                                             rule, ctx->saved_data["unit"].toDouble());
+      res[0] = dq, res[1] = dk, res[2] = dv;
+      if (t[9].defined()) res[7] = dt;
+    }
+    return once(std::move(res), "cross_attention is differentiable once on the GPU (use composite_mode)");
+  }
+};
+
+static bool wants(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
+
+static at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                  const at::Tensor& q_ptr, const at::Tensor& k_ptr, const OptTensor& mask, double scale,
+                                  const OptTensor& table, const OptTensor& q_pos, const OptTensor& k_pos,
+                                  at::IntArrayRef rule, double unit) {
+  return std::get<0>(cross_attn_fwd(q, k, v, q_ptr, k_ptr, mask, scale, table, q_pos, k_pos, rule, unit, false));
+}
+
+static at::Tensor cross_attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                           const at::Tensor& q_ptr, const at::Tensor& k_ptr, const OptTensor& mask,
+                                           double scale, const OptTensor& table, const OptTensor& q_pos,
+                                           const OptTensor& k_pos, at::IntArrayRef rule, double unit) {
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || wants(table)))
+    return CrossAttn::apply(q, k, v, q_ptr, k_ptr, mask, scale, table, q_pos, k_pos, rule.vec(), unit);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return cross_attention(q, k, v, q_ptr, k_ptr, mask, scale, table, q_pos, k_pos, rule, unit);
+}
+
 }  // namespace xa
 }  // namespace hy
 
 TORCH_LIBRARY_FRAGMENT(hydra, m) {
   m.def(
-      "cross_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor q_ptr, Tensor k_ptr, Tensor? key_mask, float scale, "
-      "Tensor? table, Tensor? q_pos, Tensor? k_pos, int[] rule, float unit, bool save) -> (Tensor, Tensor, Tensor)");
-  m.def(
-      "cross_attn_bwd(Tensor d_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor rest, Tensor lse, Tensor q_ptr, Tensor k_ptr, "
-      "Tensor? key_mask, float scale, Tensor? table, Tensor? q_pos, Tensor? k_pos, int[] rule, float unit) -> "
-      "(Tensor, Tensor, Tensor, Tensor)");
+      "cross_attention(Tensor q, Tensor k, Tensor v, Tensor q_ptr, Tensor k_ptr, Tensor? key_mask, float scale, "
+      "Tensor? table, Tensor? q_pos, Tensor? k_pos, int[] rule, float unit) -> Tensor");
 }
-TORCH_LIBRARY_IMPL(hydra, CUDA, m) {
-  m.impl("cross_attn_fwd", hy::xa::cross_attn_fwd);
-  m.impl("cross_attn_bwd", hy::xa::cross_attn_bwd);
-}
+TORCH_LIBRARY_IMPL(hydra, CUDA, m) { m.impl("cross_attention", hy::xa::cross_attention); }
+TORCH_LIBRARY_IMPL(hydra, AutogradCUDA, m) { m.impl("cross_attention", hy::xa::cross_attention_autograd); }

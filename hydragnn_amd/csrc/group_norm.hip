@@ -17,6 +17,7 @@
 // goes by atomics.
 #include <c10/core/DeviceGuard.h>
 
+#include "autograd_once.h"
 #include "ragged.h"
 
 namespace hy {
@@ -641,7 +642,7 @@ static Args fill(const at::Tensor& x, const OptTensor& w, const OptTensor& b, co
   return a;
 }
 
-std::tuple<at::Tensor, at::Tensor> group_norm_fwd(const at::Tensor& x_, const OptTensor& w, const OptTensor& b,
+static std::tuple<at::Tensor, at::Tensor> group_norm_fwd(const at::Tensor& x_, const OptTensor& w, const OptTensor& b,
                                                   const OptTensor& ptr, int64_t seqs, int64_t groups, double eps,
                                                   int64_t act, bool save) {
   HY_CHECK_CUDA(x_);
@@ -658,7 +659,7 @@ std::tuple<at::Tensor, at::Tensor> group_norm_fwd(const at::Tensor& x_, const Op
   return {y, stat};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> group_norm_bwd(const at::Tensor& dy_, const at::Tensor& x_,
+static std::tuple<at::Tensor, at::Tensor, at::Tensor> group_norm_bwd(const at::Tensor& dy_, const at::Tensor& x_,
                                                               const at::Tensor& stat, const OptTensor& w,
                                                               const OptTensor& b, const OptTensor& ptr, int64_t seqs,
                                                               int64_t groups, double eps, int64_t act) {
@@ -685,18 +686,60 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> group_norm_bwd(const at::Tensor& 
   return {dx, dw, db};
 }
 
+struct GroupNorm : public torch::autograd::Function<GroupNorm> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const OptTensor& w,
+                            const OptTensor& b, const OptTensor& ptr, int64_t seqs, int64_t groups, double eps,
+                            int64_t act) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, stat] = group_norm_fwd(x, w, b, ptr, seqs, groups, eps, act, true);
+    auto some = [](const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); };
+    ctx->save_for_backward({x, stat, some(w), some(b), some(ptr)});
+    ctx->saved_data["seqs"] = seqs;
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["act"] = act;
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    auto some = [](const at::Tensor& x) { return x.defined() ? OptTensor(x) : OptTensor(); };
+    torch::autograd::variable_list res(8);
+    if (!grads[0].defined()) return res;
+    {
+      at::AutoGradMode off(false);
+      auto [dx, dw, db] = group_norm_bwd(grads[0], t[0], t[1], some(t[2]), some(t[3]), some(t[4]),
+                                         ctx->saved_data["seqs"].toInt(), ctx->saved_data["groups"].toInt(),
+                                         ctx->saved_data["eps"].toDouble(), ctx->saved_data["act"].toInt());
+      res[0] = dx;
+      if (t[2].defined()) res[1] = dw;
+      if (t[3].defined()) res[2] = db;
+    }
+    return once(std::move(res), "group_norm is differentiable once on the GPU (use composite_mode)");
+  }
+};
+
+static at::Tensor group_norm(const at::Tensor& x, const OptTensor& w, const OptTensor& b, const OptTensor& ptr,
+                             int64_t seqs, int64_t groups, double eps, int64_t act) {
+  return std::get<0>(group_norm_fwd(x, w, b, ptr, seqs, groups, eps, act, false));
+}
+
+static at::Tensor group_norm_autograd(const at::Tensor& x, const OptTensor& w, const OptTensor& b,
+                                      const OptTensor& ptr, int64_t seqs, int64_t groups, double eps, int64_t act) {
+  auto wants = [](const OptTensor& t) { return t.has_value() && t->requires_grad(); };
+  if (at::GradMode::is_enabled() && (x.requires_grad() || wants(w) || wants(b)))
+    return GroupNorm::apply(x, w, b, ptr, seqs, groups, eps, act);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return group_norm(x, w, b, ptr, seqs, groups, eps, act);
+}
+
 }  // namespace gn
 }  // namespace hy
 
 TORCH_LIBRARY_FRAGMENT(hydra, m) {
   m.def(
-      "group_norm_fwd(Tensor x, Tensor? weight, Tensor? bias, Tensor? ptr, int seqs, int groups, float eps, int act, "
-      "bool save) -> (Tensor, Tensor)");
-  m.def(
-      "group_norm_bwd(Tensor dy, Tensor x, Tensor stat, Tensor? weight, Tensor? bias, Tensor? ptr, int seqs, "
-      "int groups, float eps, int act) -> (Tensor, Tensor, Tensor)");
+      "group_norm(Tensor x, Tensor? weight, Tensor? bias, Tensor? ptr, int seqs, int groups, float eps, int act) -> "
+      "Tensor");
 }
-TORCH_LIBRARY_IMPL(hydra, CUDA, m) {
-  m.impl("group_norm_fwd", hy::gn::group_norm_fwd);
-  m.impl("group_norm_bwd", hy::gn::group_norm_bwd);
-}
+TORCH_LIBRARY_IMPL(hydra, CUDA, m) { m.impl("group_norm", hy::gn::group_norm); }
+TORCH_LIBRARY_IMPL(hydra, AutogradCUDA, m) { m.impl("group_norm", hy::gn::group_norm_autograd); }

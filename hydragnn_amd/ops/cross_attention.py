@@ -14,7 +14,6 @@ import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native
 from . import pna as _mode
@@ -140,25 +139,6 @@ def _check(q, k, v, q_ptr, k_ptr, key_mask, table, buckets, q_pos, k_pos):
         raise ValueError("cross_attention: positions without a table")
 
 
-class _CrossAttn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, q_ptr, k_ptr, key_mask, scale, table, q_pos, k_pos, rule, unit):
-        out, rest, lse = _native.ops().cross_attn_fwd(q, k, v, q_ptr, k_ptr, key_mask, scale, table, q_pos, k_pos,
-                                                      rule, unit, True)
-        ctx.save_for_backward(q, k, v, out, rest, lse, q_ptr, k_ptr, key_mask, table, q_pos, k_pos)
-        ctx.cfg = scale, rule, unit
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_out):
-        q, k, v, out, rest, lse, q_ptr, k_ptr, key_mask, table, q_pos, k_pos = ctx.saved_tensors
-        scale, rule, unit = ctx.cfg
-        dq, dk, dv, dt = _native.ops().cross_attn_bwd(d_out, q, k, v, out, rest, lse, q_ptr, k_ptr, key_mask, scale,
-                                                      table, q_pos, k_pos, rule, unit)
-        return dq, dk, dv, None, None, None, None, None if table is None else dt, None, None, None, None
-
-
 def cross_attention(q, k, v, q_ptr, k_ptr, scale=None, key_mask=None, table=None, buckets=None, q_pos=None,
                     k_pos=None):
     """Attention of ``q`` [Nq, H, D] on ``k``, ``v`` [Nk, Hk, D] -> [Nq, H, D].
@@ -189,11 +169,7 @@ def cross_attention(q, k, v, q_ptr, k_ptr, scale=None, key_mask=None, table=None
     if key_mask is not None:
         key_mask = key_mask.contiguous()
     q_ptr, k_ptr = q_ptr.contiguous(), k_ptr.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                    or (table is not None and table.requires_grad)):
-        return _CrossAttn.apply(q, k, v, q_ptr, k_ptr, key_mask, scale, table, q_pos, k_pos, rule, unit)
-    return _native.ops().cross_attn_fwd(q, k, v, q_ptr, k_ptr, key_mask, scale, table, q_pos, k_pos, rule, unit,
-                                        False)[0]
+    return _native.ops().cross_attention(q, k, v, q_ptr, k_ptr, key_mask, scale, table, q_pos, k_pos, rule, unit)
 
 
 def _attend(q, k, v, scale, bias):

@@ -13,7 +13,6 @@ GPU training mode runs the two-pass HIP kernels of ``csrc/batchnorm.hip``
 """
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from .. import _native
 from . import pna as _mode
@@ -152,22 +151,6 @@ _ACTS = {"none": 0, "relu": 1, "silu": 2}
 GROUP_NORM_MAX_CHANNELS = 4096
 
 
-class _GroupNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, ptr, seqs, groups, eps, act):
-        y, stat = _native.ops().group_norm_fwd(x, weight, bias, ptr, seqs, groups, eps, act, True)
-        ctx.save_for_backward(x, stat, weight, bias, ptr)
-        ctx.cfg = seqs, groups, eps, act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, stat, weight, bias, ptr = ctx.saved_tensors
-        dx, dw, db = _native.ops().group_norm_bwd(dy, x, stat, weight, bias, ptr, *ctx.cfg)
-        return dx, dw if weight is not None else None, db if bias is not None else None, None, None, None, None, None
-
-
 def _check_group_norm(x, groups, weight, bias, ptr, act):
     if x.dim() < 2:
         raise ValueError("group_norm: x is [rows, channels] or [samples, ..., channels]")
@@ -218,11 +201,7 @@ def group_norm(x, groups, weight=None, bias=None, ptr=None, eps=1e-5, act="none"
     else:
         ptr = ptr.contiguous()
     w, b = (None if p is None else p.float().contiguous() for p in (weight, bias))
-    if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)
-                                    or (b is not None and b.requires_grad)):
-        y = _GroupNorm.apply(x, w, b, ptr, seqs, groups, float(eps), _ACTS[act])
-    else:
-        y = _native.ops().group_norm_fwd(x, w, b, ptr, seqs, groups, float(eps), _ACTS[act], False)[0]
+    y = _native.ops().group_norm(x, w, b, ptr, seqs, groups, float(eps), _ACTS[act])
     return y if y.shape == shape else y.view(shape)
 
 
