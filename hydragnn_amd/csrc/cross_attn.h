@@ -35,7 +35,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaxBuckets = 64;  // the gradient keeps one column a lane of a [buckets, 64] table in LDS
 constexpr int kMaxFar = 2048;    // the bias is looked up by whole distance in LDS
-constexpr int kTile = 64;        // rows of the operand that is streamed through LDS
+
+// Rows of the operands that are streamed through LDS: 64, or 32 where a tile of 64 rows on its way
+// there would take 32 registers a thread and more (float from 64 columns on), and spill others.
+template <typename T, int DP>
+constexpr int kTileOf = sizeof(T) * DP >= 256 && sizeof(T) == 4 ? 32 : 64;
 
 enum Bias { kNoBias = 0, kOrder = 1, kSpace = 2 };
 
@@ -57,7 +61,7 @@ struct Args {
   const int *q_ptr, *k_ptr;
   const uint8_t* key_mask;
   int Nq, Nk, S, H, Hk, G, D;
-  int vec_q, vec_k, vec_v, vec_do;  // rows may be read 16 bytes at a time
+  int unit_q, unit_k, unit_v, unit_do, unit_o;  // bytes that rows may be read by at once (load16)
   float scale;
   void* out;    // [Nq, H, D]
   void* rest;   // [Nq, H, D], 16-bit types in training: what the rounding of `out` leaves.  The backward's
@@ -101,22 +105,45 @@ struct El<_Float16> {
   }
 };
 
-// 16 bytes of row `p` from column d0 on; zeros behind column D (and where !ok)
+// Loads go through buffer descriptors on a tile's first row: what is not there is asked for behind
+// the descriptor's range and comes back as zeros, so a tile's edge, a mask and a head width that is
+// no multiple of 16 bytes cost no branch.
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+constexpr int kNowhere = (int)0x80000000u;
+
+__device__ __forceinline__ Rsrc rsrc_of(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0x7fffffff, 0x00020000);
+}
+
+// 16 bytes at column d0 of the row that begins at byte `at`; zeros behind column D.  `unit`: the
+// bytes that every row may be read by at once (16, 8, 4 or 2; the same for a whole launch).
 template <typename T>
-__device__ __forceinline__ uint4 load16(const T* p, int d0, int D, bool ok, bool vec) {
-  uint4 r = make_uint4(0, 0, 0, 0);
-  if (!ok || d0 >= D) return r;
-  if (vec) return *reinterpret_cast<const uint4*>(p + d0);
-  constexpr int kPer = El<T>::kPer;
-  union {
-    uint4 u;
-    T e[kPer];
-  } x;
-  x.u = r;
+__device__ __forceinline__ u4 load16(Rsrc r, int at, int d0, int D, bool ok, int unit) {
+  const int off = at + d0 * (int)sizeof(T), left = ok ? (D - d0) * (int)sizeof(T) : 0;  // bytes of the row
+  u4 x;
+  if (unit == 16) return __builtin_amdgcn_raw_buffer_load_b128(r, left > 0 ? off : kNowhere, 0, 0);
+  if (unit == 8) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (d0 + i < D) x.e[i] = p[d0 + i];
-  return x.u;
+    for (int i = 0; i < 2; ++i) {
+      const u2 y = __builtin_amdgcn_raw_buffer_load_b64(r, left > 8 * i ? off + 8 * i : kNowhere, 0, 0);
+      x[2 * i] = y[0];
+      x[2 * i + 1] = y[1];
+    }
+  } else if (unit == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = __builtin_amdgcn_raw_buffer_load_b32(r, left > 4 * i ? off + 4 * i : kNowhere, 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned lo = __builtin_amdgcn_raw_buffer_load_b16(r, left > 4 * i ? off + 4 * i : kNowhere, 0, 0);
+      const unsigned hi = __builtin_amdgcn_raw_buffer_load_b16(r, left > 4 * i + 2 ? off + 4 * i + 2 : kNowhere, 0, 0);
+      x[i] = lo | (hi << 16);
+    }
+  }
+  return x;
 }
 
 // One operand of width DP (the head width rounded up) in LDS or registers.
@@ -137,14 +164,16 @@ struct Mat {
     for (int j = 0; j < RF; ++j) x.f[j] = *reinterpret_cast<const v8*>(row + 32 * j + 8 * g);
     return x;
   }
-  static __device__ __forceinline__ Row row_global(const T* row, int g, int D, bool ok, bool vec) {
+  static __device__ __forceinline__ Row row_global(Rsrc r, int at, int g, int D, bool ok, int unit) {
     Row x;
 #pragma unroll
-    for (int j = 0; j < RF; ++j) {
-      const uint4 u = load16(row, 32 * j + 8 * g, D, ok, vec);
-      x.f[j] = __builtin_bit_cast(v8, u);
-    }
+    for (int j = 0; j < RF; ++j) x.f[j] = __builtin_bit_cast(v8, load16<T>(r, at, 32 * j + 8 * g, D, ok, unit));
     return x;
+  }
+  static __device__ __forceinline__ void negate(Row& x) {
+#pragma unroll
+    for (int j = 0; j < RF; ++j)
+      x.f[j] = __builtin_bit_cast(v8, __builtin_bit_cast(u4, x.f[j]) ^ u4(0x80008000u));
   }
   static __device__ __forceinline__ f4 dot(const Row& a, const Row& b, f4 acc) {
 #pragma unroll
@@ -219,11 +248,15 @@ struct Mat<float, DP> {
     for (int j = 0; j < RF; ++j) x.f[j] = *reinterpret_cast<const f4*>(row + 16 * j + 4 * g);
     return x;
   }
-  static __device__ __forceinline__ Row row_global(const float* row, int g, int D, bool ok, bool vec) {
+  static __device__ __forceinline__ Row row_global(Rsrc r, int at, int g, int D, bool ok, int unit) {
     Row x;
 #pragma unroll
-    for (int j = 0; j < RF; ++j) x.f[j] = __builtin_bit_cast(f4, load16(row, 16 * j + 4 * g, D, ok, vec));
+    for (int j = 0; j < RF; ++j) x.f[j] = __builtin_bit_cast(f4, load16<float>(r, at, 16 * j + 4 * g, D, ok, unit));
     return x;
+  }
+  static __device__ __forceinline__ void negate(Row& x) {
+#pragma unroll
+    for (int j = 0; j < RF; ++j) x.f[j] = -x.f[j];
   }
   static __device__ __forceinline__ f4 dot(const Row& a, const Row& b, f4 acc) {
 #pragma unroll
@@ -283,30 +316,48 @@ struct Mat<float, DP> {
   }
 };
 
-// One streamed operand's tile of kTile rows on its way from memory to LDS: 256 threads, 16 bytes
-// each, held in registers while the tile before it is worked on.  Rows outside [., end) and masked
+// One streamed operand's tile on its way from memory to LDS: 256 threads, 16 bytes
+// each, held in registers while the tile before it is worked on.  Rows behind the sequence and masked
 // ones become zeros, so that whatever they hold (infinities, NaN) meets no product.
 template <typename T, int DP>
 struct Stage {
   static constexpr int kPer = El<T>::kPer;
-  static constexpr int CPR = DP / kPer;                  // 16-byte chunks of a row
-  static constexpr int CH = kTile * CPR / 256;           // of one thread
-  static_assert(kTile * CPR % 256 == 0, "a tile is a whole number of chunks a thread");
-  uint4 r[CH];
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int end, const uint8_t* mask, int D,
-                                       bool vec, int tid) {
+  static constexpr int TK = kTileOf<T, DP>;
+  static constexpr int CPR = DP / kPer;      // 16-byte chunks of a row
+  static constexpr int CH = TK * CPR / 256;  // of one thread
+  static_assert(TK * CPR % 256 == 0, "a tile is a whole number of chunks a thread");
+  struct Keep {  // which of a thread's rows take part
+    unsigned m[CH];
+  };
+  u4 r[CH];
+  // base: the tile's first row; rows: how many of it are there
+  static __device__ __forceinline__ void keep(Keep& k, const uint8_t* mask, int row0, int rows, int tid) {
+    if (mask == nullptr) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) k.m[c] = 1;
+      return;
+    }
+    const Rsrc r = rsrc_of(mask + row0);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int i = tid + c * 256, row = row0 + i / CPR;
-      const bool ok = row < end && (mask == nullptr || mask[row] != 0);
-      r[c] = load16(base + (int64_t)row * stride, (i % CPR) * kPer, D, ok, vec);
+      const int row = (tid + c * 256) / CPR;
+      k.m[c] = __builtin_amdgcn_raw_buffer_load_b8(r, row < rows ? row : kNowhere, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int rows, const Keep& k, int D, int unit,
+                                       int tid) {
+    const Rsrc rs = rsrc_of(base + (int64_t)row0 * stride);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = tid + c * 256, row = i / CPR;
+      r[c] = load16<T>(rs, row * (int)(stride * sizeof(T)), (i % CPR) * kPer, D, row < rows && k.m[c] != 0, unit);
     }
   }
   __device__ __forceinline__ void store(T* lds, int tid) const {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int i = tid + c * 256;
-      *reinterpret_cast<uint4*>(lds + (i / CPR) * Mat<T, DP>::LD + (i % CPR) * kPer) = r[c];
+      *reinterpret_cast<u4*>(lds + (i / CPR) * Mat<T, DP>::LD + (i % CPR) * kPer) = r[c];
     }
   }
 };
@@ -377,18 +428,43 @@ __device__ __forceinline__ int space_index(float qx, float qy, float qz, float k
   return i;
 }
 
-// Keys' or queries' positions of one streamed tile in LDS (int: one array; space: three).
-template <int BIAS>
-__device__ __forceinline__ void stage_pos(int* lds, const void* pos, int row0, int end, int tid) {
-  if constexpr (BIAS == kOrder) {
-    if (tid < kTile) lds[tid] = row0 + tid < end ? ((const int*)pos)[row0 + tid] : 0;
-  } else if constexpr (BIAS == kSpace) {
-    if (tid < 3 * kTile) {
-      const int row = tid / 3, c = tid - 3 * row;
-      ((float*)lds)[c * kTile + row] = row0 + row < end ? ((const float*)pos)[(int64_t)(row0 + row) * 3 + c] : 0.f;
+// Positions of one streamed tile on their way to LDS (order: one array of TK; space: three).
+template <int BIAS, int TK>
+struct StagePos {
+  unsigned v;
+  __device__ __forceinline__ void load(const void* pos, int row0, int rows, int tid) {
+    if constexpr (BIAS == kOrder) {
+      v = __builtin_amdgcn_raw_buffer_load_b32(rsrc_of((const int*)pos + row0), tid < rows ? 4 * tid : kNowhere, 0, 0);
+    } else if constexpr (BIAS == kSpace) {
+      v = __builtin_amdgcn_raw_buffer_load_b32(rsrc_of((const float*)pos + (int64_t)row0 * 3),
+                                               tid < 3 * rows ? 4 * tid : kNowhere, 0, 0);
     }
   }
-}
+  __device__ __forceinline__ void store(int* lds, int tid) const {
+    if constexpr (BIAS == kOrder) {
+      if (tid < TK) lds[tid] = (int)v;
+    } else if constexpr (BIAS == kSpace) {
+      if (tid < 3 * TK) lds[(tid % 3) * TK + tid / 3] = (int)v;
+    }
+  }
+};
+
+// One of the two LDS buffers of a streamed tile: two operands, NF rows of TK floats, positions.
+template <typename T, int DP, int NF>
+struct Tiles {
+  static constexpr int TK = kTileOf<T, DP>;
+  static constexpr int kOp = TK * Mat<T, DP>::LD;
+  static constexpr size_t kBytes = 2 * kOp * sizeof(T) + (NF + 3) * TK * 4;
+  T *a, *b;
+  float* f;
+  int* pos;
+  __device__ __forceinline__ Tiles(uint8_t* smem, int buf) {
+    a = (T*)(smem + buf * kBytes);
+    b = a + kOp;
+    f = (float*)(b + kOp);
+    pos = (int*)(f + NF * TK);
+  }
+};
 
 struct Pos {  // one row's position
   int i;
@@ -407,6 +483,44 @@ __device__ __forceinline__ Pos load_pos(const void* pos, int row, bool ok) {
     p.z = f[2];
   }
   return p;
+}
+
+// Look-up entries of the four pairs of tile rows at..at + 3 with a lane's own row.  FLIP: the tile
+// holds the queries.
+template <int BIAS, int TK, bool FLIP = false>
+struct Index {
+  int i[4];
+  __device__ __forceinline__ Index(const int* pos, int at, const Pos& own, const Rule& rule) {
+    if constexpr (BIAS == kOrder) {
+      const int4 p = *reinterpret_cast<const int4*>(pos + at);
+      const int t[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) i[r] = FLIP ? order_index(own.i, t[r], rule.far) : order_index(t[r], own.i, rule.far);
+    } else if constexpr (BIAS == kSpace) {
+      const float* p = (const float*)pos + at;
+      const f4 x = *(const f4*)p, y = *(const f4*)(p + TK), z = *(const f4*)(p + 2 * TK);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) i[r] = space_index(own.x, own.y, own.z, x[r], y[r], z[r], rule);
+    }
+  }
+};
+
+// A product as an exponent of 2, with its bias and its key's 0 or -inf.  One form for all passes, so
+// that the backward's p are the forward's.
+template <int BIAS>
+__device__ __forceinline__ float score(float x, float c, const float* lut, int i, float off) {
+  if constexpr (BIAS == kNoBias) return fmaf(x, c, off);
+  return fmaf(x, c, lut[i]) + off;
+}
+
+// A float added in LDS without a wait for it.  Only one lane ever adds to an address, so the order of
+// its sum is the lane's own.
+__device__ __forceinline__ void lds_add(float* p, float x) {
+  __hip_atomic_fetch_add(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+}
+
+inline void allow_lds(const void* kernel, size_t bytes) {  // above 64 KB a kernel has to be told
+  if (bytes > 65536) (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
 }  // namespace xa

@@ -9,17 +9,22 @@ namespace xa {
 
 void forward(const Args& a, at::ScalarType t, int bias, hipStream_t st);
 void backward(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st);
-int64_t table_tiles(int64_t Nq, int64_t S, at::ScalarType t);
+int64_t table_tiles(const Args& a, at::ScalarType t, int bias);
 
 typedef c10::optional<at::Tensor> OptTensor;
 
-// rows of `t` [N, H, D] may be read 16 bytes at a time
-static int vec16(const at::Tensor& t, int64_t D) {
-  const int64_t per = 16 / t.element_size();
-  return D % per == 0 && t.stride(0) % per == 0 && t.stride(1) % per == 0 && ((uintptr_t)t.data_ptr() & 15) == 0;
+// the bytes by which every row of `t` [N, H, D] may be read at once
+static int unit_of(const at::Tensor& t) {
+  const int64_t b = t.element_size();
+  const uint64_t all = (uint64_t)(t.size(2) * b) | (uint64_t)(t.stride(0) * b) | (uint64_t)(t.stride(1) * b) |
+                       (uint64_t)(uintptr_t)t.data_ptr() | 16;
+  return (int)(all & (~all + 1));
 }
 
-static at::Tensor rows(const at::Tensor& t) { return t.stride(2) == 1 || t.size(2) <= 1 ? t : t.contiguous(); }
+// as it is where its rows can be addressed, else a copy
+static at::Tensor rows(const at::Tensor& t) {
+  return t.dim() == 3 && (t.stride(2) == 1 || t.size(2) <= 1) && t.stride(0) < (1 << 20) ? t : t.contiguous();
+}
 
 // rule: [two_sided, side, near, far, thresholds...]
 static int fill(Args& a, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& q_ptr,
@@ -54,7 +59,10 @@ static int fill(Args& a, const at::Tensor& q, const at::Tensor& k, const at::Ten
   a.q_row = q.stride(0), a.q_head = q.stride(1);
   a.k_row = k.stride(0), a.k_head = k.stride(1);
   a.v_row = v.stride(0), a.v_head = v.stride(1);
-  a.vec_q = vec16(q, D), a.vec_k = vec16(k, D), a.vec_v = vec16(v, D);
+  a.unit_q = unit_of(q), a.unit_k = unit_of(k), a.unit_v = unit_of(v);
+  // rows of a tile are addressed by 31 bits from its first
+  for (const auto& x : {q, k, v})
+    HY_CHECK(x.stride(0) >= 0 && x.stride(0) < (1 << 20) && x.stride(1) >= 0, "cross_attention: row stride");
   a.q_ptr = q_ptr.data_ptr<int>();
   a.k_ptr = k_ptr.data_ptr<int>();
   a.scale = (float)scale;
@@ -143,14 +151,16 @@ static std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd
   at::Tensor dtable = bias != kNoBias ? at::empty({a.H, a.rule.buckets}, f32) : at::empty({0}, f32);
   at::Tensor delta = at::empty({a.H, a.Nq}, f32);
   at::Tensor part = bias != kNoBias
-                        ? at::empty({table_tiles(a.Nq, a.S, q.scalar_type()) * a.H * a.rule.buckets}, f32)
+                        ? at::empty({table_tiles(a, q.scalar_type(), bias) * a.H * a.rule.buckets}, f32)
                         : at::Tensor();
   a.out = out.data_ptr();
   a.rest = rest.numel() > 0 ? rest.data_ptr() : nullptr;
   a.lse = lse.data_ptr<float>();
   a.d_out = dout.data_ptr();
   a.do_row = dout.stride(0), a.do_head = dout.stride(1);
-  a.vec_do = vec16(dout, a.D);
+  a.unit_do = unit_of(dout);
+  HY_CHECK(dout.stride(0) >= 0 && dout.stride(0) < (1 << 20) && dout.stride(1) >= 0, "cross_attention: row stride");
+  a.unit_o = unit_of(out);
   a.delta = delta.data_ptr<float>();
   a.dq = dq.data_ptr();
   a.dk = dk.data_ptr();

@@ -14,15 +14,12 @@ namespace xa {
 
 // ------------------------------------------------------------------ query pass
 template <typename T, int DP, int NQ, int BIAS>
-__global__ __launch_bounds__(256) void bwd_query_kernel(Args a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void bwd_query_kernel(Args a) {
   typedef Mat<T, DP> M;
-  constexpr int ROWS = 64 * NQ;
+  typedef Tiles<T, DP, 1> L;
+  constexpr int ROWS = 64 * NQ, TK = L::TK;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  T* Ks = (T*)smem;
-  T* Vs = Ks + kTile * M::LD;
-  float* kadd = (float*)(Vs + kTile * M::LD);
-  int* kpos = (int*)(kadd + kTile);
-  float* hist = (float*)(kpos + 3 * kTile);  // [4 waves, buckets, 64 lanes]: every lane adds to its own column
+  float* hist = (float*)(smem + 2 * L::kBytes);  // [4 waves, buckets, 64 lanes]: every lane adds to its own column
   const int nb = BIAS != kNoBias ? a.rule.buckets : 0;
   float* lut = hist + 4 * nb * 64;
   const int nl = BIAS != kNoBias ? lut_size<BIAS>(a.rule) : 0;
@@ -40,39 +37,42 @@ __global__ __launch_bounds__(256) void bwd_query_kernel(Args a) {
     k0 = min(max(a.k_ptr[tile.seq], 0), a.Nk);
     k1 = min(max(a.k_ptr[tile.seq + 1], k0), a.Nk);
   }
-  const T* q = (const T*)a.q + h * a.q_head;
-  const T* dout = (const T*)a.d_out + h * a.do_head;
   const T* k = (const T*)a.k + (h / a.G) * a.k_head;
   const T* v = (const T*)a.v + (h / a.G) * a.v_head;
 
-  const int r0 = tile.start + wave * 16 * NQ;
-  const bool active = r0 < tile.end;
+  const int r0 = wave * 16 * NQ, rows = tile.end - tile.start;
+  const bool active = r0 < rows;
   typename M::Row qf[NQ], df[NQ];
   Pos qp[NQ];
   f4 dq[NQ][M::DT];
   float lse[NQ], delta[NQ];
+  {
+    const Rsrc rq = rsrc_of((const T*)a.q + h * a.q_head + (int64_t)tile.start * a.q_row);
+    const Rsrc rd = rsrc_of((const T*)a.d_out + h * a.do_head + (int64_t)tile.start * a.do_row);
+    const int64_t o_row = (int64_t)a.H * a.D, o_at = (int64_t)h * a.D + (int64_t)tile.start * o_row;
+    const Rsrc ro = rsrc_of((const T*)a.out + o_at), re = rsrc_of((const T*)a.rest + o_at);
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int row = r0 + 16 * n + li;
-    const bool ok = row < tile.end;
-    qf[n] = M::row_global(q + (int64_t)row * a.q_row, g, a.D, ok, a.vec_q);
-    df[n] = M::row_global(dout + (int64_t)row * a.do_row, g, a.D, ok, a.vec_do);
-    qp[n] = load_pos<BIAS>(a.q_pos, row, ok);
-    const bool vec_o = a.D % El<T>::kPer == 0;
-    const typename M::Row of = M::row_global((const T*)a.out + ((int64_t)row * a.H + h) * a.D, g, a.D, ok, vec_o);
-    // the diagonal of O dO^T, by the very products that give dP: a row with one key has o = v, so its
-    // dP - delta is zero and not the rounding of two orders of one sum
-    f4 od = M::dot(of, df[n], f4{0.f, 0.f, 0.f, 0.f});
-    if (a.rest != nullptr)
-      od = M::dot(M::row_global((const T*)a.rest + ((int64_t)row * a.H + h) * a.D, g, a.D, ok, vec_o), df[n], od);
-    float mine = 0.f;
+    for (int n = 0; n < NQ; ++n) {
+      const int row = r0 + 16 * n + li;
+      const bool ok = row < rows;
+      qf[n] = M::row_global(rq, row * (int)(a.q_row * sizeof(T)), g, a.D, ok, a.unit_q);
+      df[n] = M::row_global(rd, row * (int)(a.do_row * sizeof(T)), g, a.D, ok, a.unit_do);
+      qp[n] = load_pos<BIAS>(a.q_pos, tile.start + row, ok);
+      // the diagonal of O dO^T, by the very products that give dP: a row with one key has o = v, so its
+      // dP - delta is zero and not the rounding of two orders of one sum
+      const int at = row * (int)(o_row * sizeof(T));
+      f4 od = M::dot(M::row_global(ro, at, g, a.D, ok, a.unit_o), df[n], f4{0.f, 0.f, 0.f, 0.f});
+      if (sizeof(T) == 2) od = M::dot(M::row_global(re, at, g, a.D, ok, a.unit_o), df[n], od);
+      float mine = 0.f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) mine = li == 4 * g + r ? od[r] : mine;
-    delta[n] = column_sum(mine);
-    lse[n] = ok ? a.lse[(int64_t)h * a.Nq + row] : INFINITY;  // exp2(z - inf): a row that is not there has no p
-    if (ok && g == 0) a.delta[(int64_t)h * a.Nq + row] = delta[n];
+      for (int r = 0; r < 4; ++r) mine = li == 4 * g + r ? od[r] : mine;
+      delta[n] = column_sum(mine);
+      const int64_t to = (int64_t)h * a.Nq + tile.start + row;
+      lse[n] = ok ? a.lse[to] : INFINITY;  // exp2(z - inf): a row that is not there has no p
+      if (ok && g == 0) a.delta[to] = delta[n];
 #pragma unroll
-    for (int d = 0; d < M::DT; ++d) dq[n][d] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int d = 0; d < M::DT; ++d) dq[n][d] = f4{0.f, 0.f, 0.f, 0.f};
+    }
   }
   if constexpr (BIAS != kNoBias) {
     const float* tab = (const float*)a.table + h * nb;
@@ -86,73 +86,78 @@ __global__ __launch_bounds__(256) void bwd_query_kernel(Args a) {
   const float c = a.scale * kLog2e;
 
   Stage<T, DP> sk, sv;
+  typename Stage<T, DP>::Keep keep;
+  StagePos<BIAS, TK> sp;
+  float add = 0.f;
+  auto fetch = [&](int kt) {
+    sk.load(k, a.k_row, kt, k1 - kt, keep, a.D, a.unit_k, tid);
+    sv.load(v, a.v_row, kt, k1 - kt, keep, a.D, a.unit_v, tid);
+    sp.load(a.k_pos, kt, k1 - kt, tid);
+  };
+  auto masks = [&](int kt) {
+    Stage<T, DP>::keep(keep, a.key_mask, kt, k1 - kt, tid);
+    add = tid < k1 - kt && (a.key_mask == nullptr || a.key_mask[kt + (tid & (TK - 1))] != 0) ? 0.f : -INFINITY;
+  };
+  auto put = [&](int buf, float flag) {
+    const L t(smem, buf);
+    sk.store(t.a, tid);
+    sv.store(t.b, tid);
+    sp.store(t.pos, tid);
+    if (tid < TK) t.f[tid] = flag;
+  };
   if (k0 < k1) {
-    sk.load(k, a.k_row, k0, k1, a.key_mask, a.D, a.vec_k, tid);
-    sv.load(v, a.v_row, k0, k1, a.key_mask, a.D, a.vec_v, tid);
+    masks(k0);
+    fetch(k0);
+    put(0, add);
+    masks(min(k0 + TK, k1));
   }
-  for (int kt = k0; kt < k1; kt += kTile) {
+  int buf = 0;
+  for (int kt = k0; kt < k1; kt += TK, buf ^= 1) {
     __syncthreads();
-    sk.store(Ks, tid);
-    sv.store(Vs, tid);
-    if (tid < kTile) {
-      const int row = kt + tid;
-      kadd[tid] = row < k1 && (a.key_mask == nullptr || a.key_mask[row] != 0) ? 0.f : -INFINITY;
+    const bool more = kt + TK < k1;
+    const float flag = add;
+    if (more) {
+      fetch(kt + TK);
+      masks(min(kt + 2 * TK, k1));
     }
-    stage_pos<BIAS>(kpos, a.k_pos, kt, k1, tid);
-    __syncthreads();
-    if (kt + kTile < k1) {
-      sk.load(k, a.k_row, kt + kTile, k1, a.key_mask, a.D, a.vec_k, tid);
-      sv.load(v, a.v_row, kt + kTile, k1, a.key_mask, a.D, a.vec_v, tid);
-    }
-    if (!active) continue;
-    const bool some = a.key_mask != nullptr || kt + kTile > k1;
+    const L t(smem, buf);
+    if (active) {
 #pragma unroll
-    for (int u = 0; u < kTile / 32; ++u) {
-      f4 ds[2][NQ];
+      for (int u = 0; u < TK / 32; ++u) {
+        f4 ds[2][NQ];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int at = 32 * u + 16 * t;
-        const typename M::Row kf = M::row_lds(Ks + (at + li) * M::LD, g);
-        const typename M::Row vf = M::row_lds(Vs + (at + li) * M::LD, g);
+        for (int w = 0; w < 2; ++w) {
+          const int at = 32 * u + 16 * w;
+          const typename M::Row kf = M::row_lds(t.a + (at + li) * M::LD, g);
+          const typename M::Row vf = M::row_lds(t.b + (at + li) * M::LD, g);
+          const f4 off = *reinterpret_cast<const f4*>(t.f + at + 4 * g);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          f4 x = M::dot(kf, qf[n], f4{0.f, 0.f, 0.f, 0.f}) * c;
-          const f4 dp = M::dot(vf, df[n], f4{0.f, 0.f, 0.f, 0.f});
-          int e[4];
-          if constexpr (BIAS == kOrder) {
-            const int4 kp = *reinterpret_cast<const int4*>(kpos + at + 4 * g);
-            e[0] = order_index(kp.x, qp[n].i, a.rule.far);
-            e[1] = order_index(kp.y, qp[n].i, a.rule.far);
-            e[2] = order_index(kp.z, qp[n].i, a.rule.far);
-            e[3] = order_index(kp.w, qp[n].i, a.rule.far);
-          } else if constexpr (BIAS == kSpace) {
-            const float* kp = (const float*)kpos + at + 4 * g;
-            const f4 kx = *(const f4*)kp, ky = *(const f4*)(kp + kTile), kz = *(const f4*)(kp + 2 * kTile);
+          for (int n = 0; n < NQ; ++n) {
+            const f4 x = M::dot(kf, qf[n], f4{0.f, 0.f, 0.f, 0.f});
+            const f4 dp = M::dot(vf, df[n], f4{0.f, 0.f, 0.f, 0.f});
+            const Index<BIAS, TK> e(t.pos, at + 4 * g, qp[n], a.rule);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              e[r] = space_index(qp[n].x, qp[n].y, qp[n].z, kx[r], ky[r], kz[r], a.rule);
-          }
-          if constexpr (BIAS != kNoBias) {
+              ds[w][n][r] = __builtin_amdgcn_exp2f(score<BIAS>(x[r], c, lut, e.i[r], off[r]) - lse[n]) *
+                            (dp[r] - delta[n]);
+            if constexpr (BIAS != kNoBias) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] += lut[e[r]];
-          }
-          if (some) x += *reinterpret_cast<const f4*>(kadd + at + 4 * g);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) ds[t][n][r] = __builtin_amdgcn_exp2f(x[r] - lse[n]) * (dp[r] - delta[n]);
-          if constexpr (BIAS != kNoBias) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) hist[(wave * nb + lutb[e[r]]) * 64 + lane] += ds[t][n][r];
+              for (int r = 0; r < 4; ++r)
+                lds_add(hist + (wave * nb + lutb[e.i[r]]) * 64 + lane, ds[w][n][r]);
+            }
           }
         }
+        M::template outer<NQ, false>(t.a + 32 * u * M::LD, ds[0], ds[1], dq, lane);
       }
-      M::template outer<NQ, false>(Ks + 32 * u * M::LD, ds[0], ds[1], dq, lane);
     }
+    if (more) put(buf ^ 1, flag);
   }
   if (active) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int row = r0 + 16 * n + li;
-      if (row < tile.end) M::store((T*)a.dq + ((int64_t)row * a.H + h) * a.D, dq[n], a.scale, a.D, g);
+      if (row < rows)
+        M::store((T*)a.dq + ((int64_t)(tile.start + row) * a.H + h) * a.D, dq[n], a.scale, a.D, g);
     }
   }
   if constexpr (BIAS != kNoBias) {
@@ -178,16 +183,12 @@ __global__ __launch_bounds__(64) void bwd_table_kernel(const float* part, float*
 
 // ------------------------------------------------------------------ key pass
 template <typename T, int DP, int NK, int BIAS>
-__global__ __launch_bounds__(256) void bwd_key_kernel(Args a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void bwd_key_kernel(Args a) {
   typedef Mat<T, DP> M;
-  constexpr int ROWS = 64 * NK;
+  typedef Tiles<T, DP, 2> L;
+  constexpr int ROWS = 64 * NK, TK = L::TK;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  T* Qs = (T*)smem;
-  T* Ds = Qs + kTile * M::LD;
-  float* qlse = (float*)(Ds + kTile * M::LD);
-  float* qdel = qlse + kTile;
-  int* qpos = (int*)(qdel + kTile);
-  float* lut = (float*)(qpos + 3 * kTile);
+  float* lut = (float*)(smem + 2 * L::kBytes);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, li = lane & 15;
   const int hk = blockIdx.x % a.Hk;
@@ -198,163 +199,179 @@ __global__ __launch_bounds__(256) void bwd_key_kernel(Args a) {
     q0 = min(max(a.q_ptr[tile.seq], 0), a.Nq);
     q1 = min(max(a.q_ptr[tile.seq + 1], q0), a.Nq);
   }
-  const T* k = (const T*)a.k + hk * a.k_head;
-  const T* v = (const T*)a.v + hk * a.v_head;
-  const int r0 = tile.start + wave * 16 * NK;
-  const bool active = r0 < tile.end;
+  const int r0 = wave * 16 * NK, rows = tile.end - tile.start;
+  const bool active = r0 < rows;
   typename M::Row kf[NK], vf[NK];
   Pos kp[NK];
-  bool keep[NK];
+  float off[NK];
   f4 dk[NK][M::DT], dv[NK][M::DT];
+  {
+    const Rsrc rk = rsrc_of((const T*)a.k + hk * a.k_head + (int64_t)tile.start * a.k_row);
+    const Rsrc rv = rsrc_of((const T*)a.v + hk * a.v_head + (int64_t)tile.start * a.v_row);
 #pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    const int row = r0 + 16 * n + li;
-    const bool ok = row < tile.end;
-    keep[n] = ok && (a.key_mask == nullptr || a.key_mask[row] != 0);
-    kf[n] = M::row_global(k + (int64_t)row * a.k_row, g, a.D, keep[n], a.vec_k);
-    vf[n] = M::row_global(v + (int64_t)row * a.v_row, g, a.D, keep[n], a.vec_v);
-    kp[n] = load_pos<BIAS>(a.k_pos, row, ok);
+    for (int n = 0; n < NK; ++n) {
+      const int row = r0 + 16 * n + li;
+      const bool ok = row < rows, keep = ok && (a.key_mask == nullptr || a.key_mask[tile.start + row] != 0);
+      kf[n] = M::row_global(rk, row * (int)(a.k_row * sizeof(T)), g, a.D, keep, a.unit_k);
+      vf[n] = M::row_global(rv, row * (int)(a.v_row * sizeof(T)), g, a.D, keep, a.unit_v);
+      kp[n] = load_pos<BIAS>(a.k_pos, tile.start + row, ok);
+      off[n] = keep ? 0.f : -INFINITY;
 #pragma unroll
-    for (int d = 0; d < M::DT; ++d) dk[n][d] = dv[n][d] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int d = 0; d < M::DT; ++d) dk[n][d] = dv[n][d] = f4{0.f, 0.f, 0.f, 0.f};
+    }
   }
   const float c = a.scale * kLog2e;
-  for (int h = hk * a.G; h < (hk + 1) * a.G; ++h) {
-    const T* q = (const T*)a.q + h * a.q_head;
-    const T* dout = (const T*)a.d_out + h * a.do_head;
-    Stage<T, DP> sq, sd;
-    if (q0 < q1) {
-      sq.load(q, a.q_row, q0, q1, nullptr, a.D, a.vec_q, tid);
-      sd.load(dout, a.do_row, q0, q1, nullptr, a.D, a.vec_do, tid);
+
+  Stage<T, DP> sq, sd;
+  typename Stage<T, DP>::Keep all;
+  Stage<T, DP>::keep(all, nullptr, 0, 0, tid);
+  StagePos<BIAS, TK> sp;
+  float row_lse = INFINITY, row_delta = 0.f;
+  auto fetch = [&](int h, int qt) {
+    sq.load((const T*)a.q + h * a.q_head, a.q_row, qt, q1 - qt, all, a.D, a.unit_q, tid);
+    sd.load((const T*)a.d_out + h * a.do_head, a.do_row, qt, q1 - qt, all, a.D, a.unit_do, tid);
+    sp.load(a.q_pos, qt, q1 - qt, tid);
+    const bool ok = tid < TK && tid < q1 - qt;
+    const int64_t at = (int64_t)h * a.Nq + qt + tid;
+    row_lse = ok ? a.lse[at] : INFINITY;
+    row_delta = ok ? a.delta[at] : 0.f;
+  };
+  auto put = [&](int buf) {
+    const L t(smem, buf);
+    sq.store(t.a, tid);
+    sd.store(t.b, tid);
+    sp.store(t.pos, tid);
+    if (tid < TK) {
+      t.f[tid] = row_lse;
+      t.f[TK + tid] = row_delta;
     }
-    if constexpr (BIAS != kNoBias) {
+  };
+  const int per = (q1 - q0 + TK - 1) / TK, steps = per * a.G;  // every query head of the group in turn
+  if (steps > 0) {
+    fetch(hk * a.G, q0);
+    put(0);
+  }
+  for (int i = 0; i < steps; ++i) {
+    const int h = hk * a.G + i / per;
+    if (BIAS != kNoBias && i % per == 0) {
       __syncthreads();  // the head before is done with the look-up table
       const float* tab = (const float*)a.table + h * a.rule.buckets;
-      for (int i = tid; i < lut_size<BIAS>(a.rule); i += 256) lut[i] = tab[lut_bucket<BIAS>(a.rule, i)] * kLog2e;
+      for (int j = tid; j < lut_size<BIAS>(a.rule); j += 256) lut[j] = tab[lut_bucket<BIAS>(a.rule, j)] * kLog2e;
     }
-    for (int qt = q0; qt < q1; qt += kTile) {
-      __syncthreads();
-      sq.store(Qs, tid);
-      sd.store(Ds, tid);
-      if (tid < kTile) {
-        const int row = qt + tid;
-        qlse[tid] = row < q1 ? a.lse[(int64_t)h * a.Nq + row] : INFINITY;
-        qdel[tid] = row < q1 ? a.delta[(int64_t)h * a.Nq + row] : 0.f;
-      }
-      stage_pos<BIAS>(qpos, a.q_pos, qt, q1, tid);
-      __syncthreads();
-      if (qt + kTile < q1) {
-        sq.load(q, a.q_row, qt + kTile, q1, nullptr, a.D, a.vec_q, tid);
-        sd.load(dout, a.do_row, qt + kTile, q1, nullptr, a.D, a.vec_do, tid);
-      }
-      if (!active) continue;
+    __syncthreads();
+    const bool more = i + 1 < steps;
+    if (more) fetch(hk * a.G + (i + 1) / per, q0 + (i + 1) % per * TK);
+    const L t(smem, i & 1);
+    if (active) {
 #pragma unroll
-      for (int u = 0; u < kTile / 32; ++u) {
+      for (int u = 0; u < TK / 32; ++u) {
         f4 p[2][NK], ds[2][NK];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int at = 32 * u + 16 * t;
-          const typename M::Row qf = M::row_lds(Qs + (at + li) * M::LD, g);
-          const typename M::Row df = M::row_lds(Ds + (at + li) * M::LD, g);
-          const f4 lse = *reinterpret_cast<const f4*>(qlse + at + 4 * g);
-          const f4 del = *reinterpret_cast<const f4*>(qdel + at + 4 * g);
+        for (int w = 0; w < 2; ++w) {
+          const int at = 32 * u + 16 * w;
+          const typename M::Row qf = M::row_lds(t.a + (at + li) * M::LD, g);
+          const typename M::Row df = M::row_lds(t.b + (at + li) * M::LD, g);
+          const f4 lse = *reinterpret_cast<const f4*>(t.f + at + 4 * g);
+          const f4 del = *reinterpret_cast<const f4*>(t.f + TK + at + 4 * g);
 #pragma unroll
           for (int n = 0; n < NK; ++n) {
-            f4 x = M::dot(qf, kf[n], f4{0.f, 0.f, 0.f, 0.f}) * c;
+            const f4 x = M::dot(qf, kf[n], f4{0.f, 0.f, 0.f, 0.f});
             const f4 dp = M::dot(df, vf[n], f4{0.f, 0.f, 0.f, 0.f});
-            if constexpr (BIAS == kOrder) {
-              const int4 qp = *reinterpret_cast<const int4*>(qpos + at + 4 * g);
-              x[0] += lut[order_index(kp[n].i, qp.x, a.rule.far)];
-              x[1] += lut[order_index(kp[n].i, qp.y, a.rule.far)];
-              x[2] += lut[order_index(kp[n].i, qp.z, a.rule.far)];
-              x[3] += lut[order_index(kp[n].i, qp.w, a.rule.far)];
-            } else if constexpr (BIAS == kSpace) {
-              const float* qp = (const float*)qpos + at + 4 * g;
-              const f4 qx = *(const f4*)qp, qy = *(const f4*)(qp + kTile), qz = *(const f4*)(qp + 2 * kTile);
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                x[r] += lut[space_index(qx[r], qy[r], qz[r], kp[n].x, kp[n].y, kp[n].z, a.rule)];
-            }
+            const Index<BIAS, TK, true> e(t.pos, at + 4 * g, kp[n], a.rule);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float e = keep[n] ? __builtin_amdgcn_exp2f(x[r] - lse[r]) : 0.f;
-              p[t][n][r] = e;
-              ds[t][n][r] = e * (dp[r] - del[r]);
+              p[w][n][r] = __builtin_amdgcn_exp2f(score<BIAS>(x[r], c, lut, e.i[r], off[n]) - lse[r]);
+              ds[w][n][r] = p[w][n][r] * (dp[r] - del[r]);
             }
           }
         }
-        M::template outer<NK, false>(Ds + 32 * u * M::LD, p[0], p[1], dv, lane);
-        M::template outer<NK, false>(Qs + 32 * u * M::LD, ds[0], ds[1], dk, lane);
+        M::template outer<NK, false>(t.b + 32 * u * M::LD, p[0], p[1], dv, lane);
+        M::template outer<NK, false>(t.a + 32 * u * M::LD, ds[0], ds[1], dk, lane);
       }
     }
+    if (more) put((i + 1) & 1);
   }
   if (!active) return;
 #pragma unroll
   for (int n = 0; n < NK; ++n) {
     const int row = r0 + 16 * n + li;
-    if (row < tile.end) {
-      M::store((T*)a.dk + ((int64_t)row * a.Hk + hk) * a.D, dk[n], a.scale, a.D, g);
-      M::store((T*)a.dv + ((int64_t)row * a.Hk + hk) * a.D, dv[n], 1.f, a.D, g);
+    if (row < rows) {
+      const int64_t at = ((int64_t)(tile.start + row) * a.Hk + hk) * a.D;
+      M::store((T*)a.dk + at, dk[n], a.scale, a.D, g);
+      M::store((T*)a.dv + at, dv[n], 1.f, a.D, g);
     }
   }
 }
 
-static int query_rows(at::ScalarType t) { return t == at::kFloat ? 64 : 128; }
+// ------------------------------------------------------------------ host
+// Rows of a wave of the query pass: 32 in 16 bits, so that a fragment read from LDS feeds two
+// products, where that leaves two workgroups a compute unit; 16 with distances, whose arithmetic wants
+// the registers.  The key pass holds two accumulators a row and keeps to 16, but for narrow heads.
+static int wave_rows(at::ScalarType t, int bias, int64_t N, int64_t S, int64_t heads) {
+  if (t == at::kFloat || bias == kSpace) return 1;
+  return (N / 128 + std::min<int64_t>(S, N)) * heads >= 2 * num_cus() ? 2 : 1;
+}
 
-int64_t table_tiles(int64_t Nq, int64_t S, at::ScalarType t) { return tile_count(Nq, S, query_rows(t)); }
-
-template <typename F>
-static void allow_lds(F* kern, size_t lds) {
-  if (lds > 65536) (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+int64_t table_tiles(const Args& a, at::ScalarType t, int bias) {
+  return tile_count(a.Nq, a.S, 64 * wave_rows(t, bias, a.Nq, a.S, a.H));
 }
 
 template <typename T, int DP, int NQ, int BIAS>
-static void launch_bwd(const Args& a, float* dtable, hipStream_t st) {
-  const size_t tiles2 = 2 * kTile * Mat<T, DP>::LD * sizeof(T);
+static void launch_query(const Args& a, float* dtable, hipStream_t st) {
   const int nl = BIAS == kOrder ? 2 * a.rule.far + 1 : BIAS == kSpace ? a.rule.far + 1 : 0;
-  const int64_t qt = tile_count(a.Nq, a.S, 64 * NQ), kt = tile_count(a.Nk, a.S, 64 * NQ);
-  HY_CHECK(qt * a.H < (int64_t(1) << 31) && kt * a.Hk < (int64_t(1) << 31),
-           "cross_attention: too many tiles for one launch");
-  {
-    size_t lds = tiles2 + 4 * kTile * 4;
-    if (BIAS != kNoBias) lds += 4 * a.rule.buckets * 64 * 4 + nl * 5;
-    auto* kern = &bwd_query_kernel<T, DP, NQ, BIAS>;
-    allow_lds(kern, lds);
-    kern<<<dim3((unsigned)(qt * a.H)), 256, lds, st>>>(a);
-  }
+  const int64_t qt = tile_count(a.Nq, a.S, 64 * NQ);
+  HY_CHECK(qt * a.H < (int64_t(1) << 31), "cross_attention: too many tiles for one launch");
+  size_t lds = 2 * Tiles<T, DP, 1>::kBytes;
+  if (BIAS != kNoBias) lds += 4 * a.rule.buckets * 64 * 4 + nl * 5;
+  auto* kern = &bwd_query_kernel<T, DP, NQ, BIAS>;
+  allow_lds((const void*)kern, lds);
+  kern<<<dim3((unsigned)(qt * a.H)), 256, lds, st>>>(a);
   if (BIAS != kNoBias) {
     const int cells = a.H * a.rule.buckets;
     bwd_table_kernel<<<dim3(cells), 64, 0, st>>>(a.part, dtable, (int)qt, cells);
   }
-  {
-    const size_t lds = tiles2 + 5 * kTile * 4 + nl * 4;
-    auto* kern = &bwd_key_kernel<T, DP, NQ, BIAS>;
-    allow_lds(kern, lds);
-    kern<<<dim3((unsigned)(kt * a.Hk)), 256, lds, st>>>(a);
-  }
 }
 
-template <typename T, int DP, int NQ>
-static void pick_bias(const Args& a, int bias, float* dtable, hipStream_t st) {
-  if (bias == kNoBias) launch_bwd<T, DP, NQ, kNoBias>(a, dtable, st);
-  else if (bias == kOrder) launch_bwd<T, DP, NQ, kOrder>(a, dtable, st);
-  else launch_bwd<T, DP, NQ, kSpace>(a, dtable, st);
+template <typename T, int DP, int NK, int BIAS>
+static void launch_key(const Args& a, hipStream_t st) {
+  const int nl = BIAS == kOrder ? 2 * a.rule.far + 1 : BIAS == kSpace ? a.rule.far + 1 : 0;
+  const int64_t kt = tile_count(a.Nk, a.S, 64 * NK);
+  HY_CHECK(kt * a.Hk < (int64_t(1) << 31), "cross_attention: too many tiles for one launch");
+  const size_t lds = 2 * Tiles<T, DP, 2>::kBytes + nl * 4;
+  auto* kern = &bwd_key_kernel<T, DP, NK, BIAS>;
+  allow_lds((const void*)kern, lds);
+  kern<<<dim3((unsigned)(kt * a.Hk)), 256, lds, st>>>(a);
+}
+
+template <typename T, int DP, int BIAS>
+static void launch_bwd(const Args& a, at::ScalarType t, float* dtable, hipStream_t st) {
+  constexpr int N2 = sizeof(T) == 2 && BIAS != kSpace ? 2 : 1;
+  if (wave_rows(t, BIAS, a.Nq, a.S, a.H) == 1) launch_query<T, DP, 1, BIAS>(a, dtable, st);
+  else launch_query<T, DP, N2, BIAS>(a, dtable, st);
+  constexpr int K2 = DP <= 32 ? N2 : 1;
+  if (wave_rows(t, BIAS, a.Nk, a.S, a.Hk) == 1) launch_key<T, DP, 1, BIAS>(a, st);
+  else launch_key<T, DP, K2, BIAS>(a, st);
+}
+
+template <typename T, int DP>
+static void pick(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st) {
+  if (bias == kNoBias) launch_bwd<T, DP, kNoBias>(a, t, dtable, st);
+  else if (bias == kOrder) launch_bwd<T, DP, kOrder>(a, t, dtable, st);
+  else launch_bwd<T, DP, kSpace>(a, t, dtable, st);
+}
+
+template <typename T>
+static void pick_width(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st) {
+  if (sizeof(T) == 4 && a.D <= 16) pick<T, sizeof(T) == 4 ? 16 : 32>(a, t, bias, dtable, st);
+  else if (a.D <= 32) pick<T, 32>(a, t, bias, dtable, st);
+  else if (a.D <= 64) pick<T, 64>(a, t, bias, dtable, st);
+  else pick<T, 128>(a, t, bias, dtable, st);
 }
 
 void backward(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st) {
-  if (t == at::kFloat) {
-    if (a.D <= 16) pick_bias<float, 16, 1>(a, bias, dtable, st);
-    else if (a.D <= 32) pick_bias<float, 32, 1>(a, bias, dtable, st);
-    else if (a.D <= 64) pick_bias<float, 64, 1>(a, bias, dtable, st);
-    else pick_bias<float, 128, 1>(a, bias, dtable, st);
-  } else if (t == at::kBFloat16) {
-    if (a.D <= 32) pick_bias<__bf16, 32, 2>(a, bias, dtable, st);
-    else if (a.D <= 64) pick_bias<__bf16, 64, 2>(a, bias, dtable, st);
-    else pick_bias<__bf16, 128, 2>(a, bias, dtable, st);
-  } else {
-    if (a.D <= 32) pick_bias<_Float16, 32, 2>(a, bias, dtable, st);
-    else if (a.D <= 64) pick_bias<_Float16, 64, 2>(a, bias, dtable, st);
-    else pick_bias<_Float16, 128, 2>(a, bias, dtable, st);
-  }
+  if (t == at::kFloat) pick_width<float>(a, t, bias, dtable, st);
+  else if (t == at::kBFloat16) pick_width<__bf16>(a, t, bias, dtable, st);
+  else pick_width<_Float16>(a, t, bias, dtable, st);
 }
 
 }  // namespace xa

@@ -8,15 +8,12 @@ namespace hy {
 namespace xa {
 
 template <typename T, int DP, int NQ, int BIAS, bool SAVE>
-__global__ __launch_bounds__(256) void fwd_kernel(Args a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void fwd_kernel(Args a) {
   typedef Mat<T, DP> M;
-  constexpr int ROWS = 64 * NQ;
+  typedef Tiles<T, DP, 1> L;
+  constexpr int ROWS = 64 * NQ, TK = L::TK, KB = TK / 16;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  T* Ks = (T*)smem;
-  T* Vs = Ks + kTile * M::LD;
-  float* kadd = (float*)(Vs + kTile * M::LD);  // 0, or -inf where the key takes no part
-  int* kpos = (int*)(kadd + kTile);
-  float* lut = (float*)(kpos + 3 * kTile);
+  float* lut = (float*)(smem + 2 * L::kBytes);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, li = lane & 15;
   const int h = blockIdx.x % a.H;
@@ -27,111 +24,137 @@ __global__ __launch_bounds__(256) void fwd_kernel(Args a) {
     k0 = min(max(a.k_ptr[tile.seq], 0), a.Nk);
     k1 = min(max(a.k_ptr[tile.seq + 1], k0), a.Nk);
   }
-  const T* q = (const T*)a.q + h * a.q_head;
   const T* k = (const T*)a.k + (h / a.G) * a.k_head;
   const T* v = (const T*)a.v + (h / a.G) * a.v_head;
 
-  const int r0 = tile.start + wave * 16 * NQ;
-  const bool active = r0 < tile.end;
-  typename M::Row qf[NQ];
+  const int r0 = wave * 16 * NQ, rows = tile.end - tile.start;  // of the tile
+  const bool active = r0 < rows;
+  const float c = fabsf(a.scale) * kLog2e;  // a negative scale turns the queries' signs: the maximum is then
+  typename M::Row qf[NQ];                   // that of the products too
   Pos qp[NQ];
   f4 o[NQ][M::DT];
   float m[NQ], l[NQ];
+  {
+    const Rsrc rq = rsrc_of((const T*)a.q + h * a.q_head + (int64_t)tile.start * a.q_row);
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int row = r0 + 16 * n + li;
-    const bool ok = row < tile.end;
-    qf[n] = M::row_global(q + (int64_t)row * a.q_row, g, a.D, ok, a.vec_q);
-    qp[n] = load_pos<BIAS>(a.q_pos, row, ok);
-    m[n] = -INFINITY;
-    l[n] = 0.f;
+    for (int n = 0; n < NQ; ++n) {
+      const int row = r0 + 16 * n + li;
+      const bool ok = row < rows;
+      qf[n] = M::row_global(rq, row * (int)(a.q_row * sizeof(T)), g, a.D, ok, a.unit_q);
+      if (a.scale < 0.f) M::negate(qf[n]);
+      qp[n] = load_pos<BIAS>(a.q_pos, tile.start + row, ok);
+      m[n] = -INFINITY;
+      l[n] = 0.f;
 #pragma unroll
-    for (int d = 0; d < M::DT; ++d) o[n][d] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int d = 0; d < M::DT; ++d) o[n][d] = f4{0.f, 0.f, 0.f, 0.f};
+    }
   }
   if constexpr (BIAS != kNoBias) {
     const float* tab = (const float*)a.table + h * a.rule.buckets;
     for (int i = tid; i < lut_size<BIAS>(a.rule); i += 256) lut[i] = tab[lut_bucket<BIAS>(a.rule, i)] * kLog2e;
   }
-  const float c = a.scale * kLog2e;
 
   Stage<T, DP> sk, sv;
+  typename Stage<T, DP>::Keep keep;
+  StagePos<BIAS, TK> sp;
+  auto fetch = [&](int kt) {  // a tile's rows, with the masks that the call before has fetched
+    sk.load(k, a.k_row, kt, k1 - kt, keep, a.D, a.unit_k, tid);
+    sv.load(v, a.v_row, kt, k1 - kt, keep, a.D, a.unit_v, tid);
+    sp.load(a.k_pos, kt, k1 - kt, tid);
+  };
+  float add = 0.f;
+  auto masks = [&](int kt) {
+    Stage<T, DP>::keep(keep, a.key_mask, kt, k1 - kt, tid);
+    add = tid < k1 - kt && (a.key_mask == nullptr || a.key_mask[kt + (tid & (TK - 1))] != 0) ? 0.f : -INFINITY;
+  };
+  auto put = [&](int buf) {
+    const L t(smem, buf);
+    sk.store(t.a, tid);
+    sv.store(t.b, tid);
+    sp.store(t.pos, tid);
+  };
   if (k0 < k1) {
-    sk.load(k, a.k_row, k0, k1, a.key_mask, a.D, a.vec_k, tid);
-    sv.load(v, a.v_row, k0, k1, a.key_mask, a.D, a.vec_v, tid);
+    masks(k0);
+    if (tid < TK) L(smem, 0).f[tid] = add;
+    fetch(k0);
+    put(0);
+    masks(min(k0 + TK, k1));
   }
-  for (int kt = k0; kt < k1; kt += kTile) {
-    __syncthreads();  // the tile before is done with
-    sk.store(Ks, tid);
-    sv.store(Vs, tid);
-    if (tid < kTile) {
-      const int row = kt + tid;
-      kadd[tid] = row < k1 && (a.key_mask == nullptr || a.key_mask[row] != 0) ? 0.f : -INFINITY;
+  int buf = 0;
+  for (int kt = k0; kt < k1; kt += TK, buf ^= 1) {
+    __syncthreads();  // this tile is there, and every wave is done with the one before it
+    const bool more = kt + TK < k1;
+    const float flag = add;
+    if (more) {
+      fetch(kt + TK);
+      masks(min(kt + 2 * TK, k1));
     }
-    stage_pos<BIAS>(kpos, a.k_pos, kt, k1, tid);
-    __syncthreads();
-    if (kt + kTile < k1) {
-      sk.load(k, a.k_row, kt + kTile, k1, a.key_mask, a.D, a.vec_k, tid);
-      sv.load(v, a.v_row, kt + kTile, k1, a.key_mask, a.D, a.vec_v, tid);
-    }
-    if (!active) continue;
-    const bool some = a.key_mask != nullptr || kt + kTile > k1;
-    f4 s[kTile / 16][NQ];
+    const L t(smem, buf);
+    if (active) {
+      f4 s[KB][NQ];
 #pragma unroll
-    for (int kb = 0; kb < kTile / 16; ++kb) {
-      const typename M::Row kf = M::row_lds(Ks + (16 * kb + li) * M::LD, g);
+      for (int kb = 0; kb < KB; ++kb) {
+        const typename M::Row kf = M::row_lds(t.a + (16 * kb + li) * M::LD, g);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[kb][n] = M::dot(kf, qf[n], f4{0.f, 0.f, 0.f, 0.f});
+      }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int at = 16 * kb + 4 * g;
+        const f4 off = *reinterpret_cast<const f4*>(t.f + at);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          const Index<BIAS, TK> e(t.pos, at, qp[n], a.rule);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[kb][n][r] = score<BIAS>(s[kb][n][r], c, lut, e.i[r], off[r]);
+        }
+      }
+      float shrink[NQ];
+      bool grown = false;
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-        f4 x = M::dot(kf, qf[n], f4{0.f, 0.f, 0.f, 0.f}) * c;
-        if constexpr (BIAS == kOrder) {
-          const int4 kp = *reinterpret_cast<const int4*>(kpos + 16 * kb + 4 * g);
-          x[0] += lut[order_index(kp.x, qp[n].i, a.rule.far)];
-          x[1] += lut[order_index(kp.y, qp[n].i, a.rule.far)];
-          x[2] += lut[order_index(kp.z, qp[n].i, a.rule.far)];
-          x[3] += lut[order_index(kp.w, qp[n].i, a.rule.far)];
-        } else if constexpr (BIAS == kSpace) {
-          const float* kp = (const float*)kpos + 16 * kb + 4 * g;
-          const f4 kx = *(const f4*)kp, ky = *(const f4*)(kp + kTile), kz = *(const f4*)(kp + 2 * kTile);
+        float top = m[n];
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            x[r] += lut[space_index(qp[n].x, qp[n].y, qp[n].z, kx[r], ky[r], kz[r], a.rule)];
-        }
-        if (some) x += *reinterpret_cast<const f4*>(kadd + 16 * kb + 4 * g);
-        s[kb][n] = x;
+        for (int kb = 0; kb < KB; ++kb)
+          top = fmaxf(fmaxf(fmaxf(fmaxf(top, s[kb][n][0]), s[kb][n][1]), s[kb][n][2]), s[kb][n][3]);
+        top = column_max(top);
+        const float at = top == -INFINITY ? 0.f : top;  // no key so far: every p is exp2(-inf)
+        shrink[n] = __builtin_amdgcn_exp2f(m[n] - at);
+        grown |= top > m[n];
+        m[n] = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            s[kb][n][r] = __builtin_amdgcn_exp2f(s[kb][n][r] - at);
+            sum += s[kb][n][r];
+          }
+        // of this lane's keys; the four lanes of a row are joined at the end.  (m = -inf: l is 0.)
+        l[n] = fmaf(l[n], shrink[n], sum);
       }
-    }
+      if (__any(grown)) {
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float top = m[n];
+        for (int n = 0; n < NQ; ++n) {
+          float by = shrink[n];
+          asm volatile("" : "+v"(by));  // (keeps the products inside the branch, which few tiles take)
 #pragma unroll
-      for (int kb = 0; kb < kTile / 16; ++kb)
-        top = fmaxf(top, fmaxf(fmaxf(s[kb][n][0], s[kb][n][1]), fmaxf(s[kb][n][2], s[kb][n][3])));
-      top = column_max(top);
-      const float at = top == -INFINITY ? 0.f : top;  // no key so far: every p is exp2(-inf)
-      if (__any(top > m[n])) {
-        const float shrink = __builtin_amdgcn_exp2f(m[n] - at);
-        l[n] *= shrink;
-#pragma unroll
-        for (int d = 0; d < M::DT; ++d) o[n][d] *= shrink;
-      }
-      m[n] = top;
-      float sum = 0.f;
-#pragma unroll
-      for (int kb = 0; kb < kTile / 16; ++kb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[kb][n][r] = __builtin_amdgcn_exp2f(s[kb][n][r] - at);
-          sum += s[kb][n][r];
+          for (int d = 0; d < M::DT; ++d) o[n][d] *= by;
         }
-      l[n] += sum;  // of this lane's keys; the four lanes of a row are joined at the end
-    }
+      }
 #pragma unroll
-    for (int u = 0; u < kTile / 32; ++u) 
-      M::template outer<NQ, SAVE>(Vs + 32 * u * M::LD, s[2 * u], s[2 * u + 1], o, lane);
+      for (int u = 0; u < TK / 32; ++u)
+        M::template outer<NQ, SAVE>(t.b + 32 * u * M::LD, s[2 * u], s[2 * u + 1], o, lane);
+    }
+    if (more) {
+      put(buf ^ 1);
+      if (tid < TK) L(smem, buf ^ 1).f[tid] = flag;
+    }
   }
   if (!active) return;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    const int row = r0 + 16 * n + li;
+    const int row = tile.start + r0 + 16 * n + li;
     const float sum = column_sum(l[n]);
     if (row < tile.end) {
       const int64_t at = ((int64_t)row * a.H + h) * a.D;
@@ -147,36 +170,36 @@ template <typename T, int DP, int NQ, int BIAS>
 static void launch_fwd(const Args& a, hipStream_t st) {
   const int64_t blocks = tile_count(a.Nq, a.S, 64 * NQ) * a.H;
   HY_CHECK(blocks < (int64_t(1) << 31), "cross_attention: too many query tiles for one launch");
-  size_t lds = 2 * kTile * Mat<T, DP>::LD * sizeof(T) + 4 * kTile * 4;
+  size_t lds = 2 * Tiles<T, DP, 1>::kBytes;
   if (BIAS == kOrder) lds += (2 * a.rule.far + 1) * 4;
   if (BIAS == kSpace) lds += (a.rule.far + 1) * 4;
   auto* kern = a.lse != nullptr ? &fwd_kernel<T, DP, NQ, BIAS, true> : &fwd_kernel<T, DP, NQ, BIAS, false>;
-  if (lds > 65536) (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  allow_lds((const void*)kern, lds);
   kern<<<dim3((unsigned)blocks), 256, lds, st>>>(a);
 }
 
-template <typename T, int DP, int NQ>
-static void pick_bias(const Args& a, int bias, hipStream_t st) {
+// 16 bits: 32 rows a wave, so that a key fragment read from LDS feeds two products; with distances
+// 16, whose arithmetic wants the registers.
+template <typename T, int DP>
+static void pick(const Args& a, int bias, hipStream_t st) {
+  constexpr int NQ = sizeof(T) == 2 ? 2 : 1;
   if (bias == kNoBias) launch_fwd<T, DP, NQ, kNoBias>(a, st);
   else if (bias == kOrder) launch_fwd<T, DP, NQ, kOrder>(a, st);
-  else launch_fwd<T, DP, NQ, kSpace>(a, st);
+  else launch_fwd<T, DP, 1, kSpace>(a, st);
+}
+
+template <typename T>
+static void pick_width(const Args& a, int bias, hipStream_t st) {
+  if (sizeof(T) == 4 && a.D <= 16) pick<T, sizeof(T) == 4 ? 16 : 32>(a, bias, st);
+  else if (a.D <= 32) pick<T, 32>(a, bias, st);
+  else if (a.D <= 64) pick<T, 64>(a, bias, st);
+  else pick<T, 128>(a, bias, st);
 }
 
 void forward(const Args& a, at::ScalarType t, int bias, hipStream_t st) {
-  if (t == at::kFloat) {
-    if (a.D <= 16) pick_bias<float, 16, 1>(a, bias, st);
-    else if (a.D <= 32) pick_bias<float, 32, 1>(a, bias, st);
-    else if (a.D <= 64) pick_bias<float, 64, 1>(a, bias, st);
-    else pick_bias<float, 128, 1>(a, bias, st);
-  } else if (t == at::kBFloat16) {
-    if (a.D <= 32) pick_bias<__bf16, 32, 2>(a, bias, st);
-    else if (a.D <= 64) pick_bias<__bf16, 64, 2>(a, bias, st);
-    else pick_bias<__bf16, 128, 2>(a, bias, st);
-  } else {
-    if (a.D <= 32) pick_bias<_Float16, 32, 2>(a, bias, st);
-    else if (a.D <= 64) pick_bias<_Float16, 64, 2>(a, bias, st);
-    else pick_bias<_Float16, 128, 2>(a, bias, st);
-  }
+  if (t == at::kFloat) pick_width<float>(a, bias, st);
+  else if (t == at::kBFloat16) pick_width<__bf16>(a, bias, st);
+  else pick_width<_Float16>(a, bias, st);
 }
 
 }  // namespace xa
