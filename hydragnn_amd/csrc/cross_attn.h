@@ -170,10 +170,15 @@ struct Mat {
     for (int j = 0; j < RF; ++j) x.f[j] = __builtin_bit_cast(v8, load16<T>(r, at, 32 * j + 8 * g, D, ok, unit));
     return x;
   }
-  static __device__ __forceinline__ void negate(Row& x) {
+  // The scale as an exponent of 2.  16 bits: the row keeps its values (a product with the scale would
+  // round them) but for the scale's sign, or zeros for a scale of 0, and what is left is returned.
+  static constexpr bool kScaled = false;
+  static __device__ __forceinline__ float take_scale(Row& x, float scale) {
+    const unsigned sign = scale < 0.f ? 0x80008000u : 0u, all = scale == 0.f ? 0u : ~0u;
 #pragma unroll
     for (int j = 0; j < RF; ++j)
-      x.f[j] = __builtin_bit_cast(v8, __builtin_bit_cast(u4, x.f[j]) ^ u4(0x80008000u));
+      x.f[j] = __builtin_bit_cast(v8, (__builtin_bit_cast(u4, x.f[j]) ^ u4(sign)) & u4(all));
+    return scale == 0.f ? kLog2e : fabsf(scale) * kLog2e;
   }
   static __device__ __forceinline__ f4 dot(const Row& a, const Row& b, f4 acc) {
 #pragma unroll
@@ -216,7 +221,11 @@ struct Mat {
       const int d = 16 * dt + 4 * g;
       const f4 x = acc[dt] * mul;
       const v4 y = __builtin_convertvector(x, v4);
-      const v4 z = __builtin_convertvector(x - __builtin_convertvector(y, f4), v4);
+      f4 left = x - __builtin_convertvector(y, f4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)  // below its own rounding it is the accumulators': a row with one key has none
+        left[r] = fabsf(left[r]) < 0x1p-18f * fabsf(x[r]) ? 0.f : left[r];
+      const v4 z = __builtin_convertvector(left, v4);
       if ((D & 3) == 0) {
         if (d < D) {
           *reinterpret_cast<v4*>(row + d) = y;
@@ -254,9 +263,11 @@ struct Mat<float, DP> {
     for (int j = 0; j < RF; ++j) x.f[j] = __builtin_bit_cast(f4, load16<float>(r, at, 16 * j + 4 * g, D, ok, unit));
     return x;
   }
-  static __device__ __forceinline__ void negate(Row& x) {
+  static constexpr bool kScaled = true;  // float: into the row, once, instead of into every score
+  static __device__ __forceinline__ float take_scale(Row& x, float scale) {
 #pragma unroll
-    for (int j = 0; j < RF; ++j) x.f[j] = -x.f[j];
+    for (int j = 0; j < RF; ++j) x.f[j] *= scale * kLog2e;
+    return 1.f;
   }
   static __device__ __forceinline__ f4 dot(const Row& a, const Row& b, f4 acc) {
 #pragma unroll
@@ -408,7 +419,9 @@ __device__ __forceinline__ int lut_bucket(const Rule& r, int i) {  // bucket of 
 // Entry of a pair by order: whole positions, whose difference may pass 32 bits.
 __device__ __forceinline__ int order_index(int kp, int qp, int far) {
   const int rel = __builtin_elementwise_sub_sat(kp, qp);
-  return min(max(rel, -far), far) + far;
+  int i;
+  asm("v_med3_i32 %0, %1, %2, %3" : "=v"(i) : "v"(rel), "v"(-far), "v"(far));
+  return i + far;
 }
 
 // Entry of a pair by distance: floor(dist / unit).  In fp32 first; where that lies within its own
@@ -428,6 +441,28 @@ __device__ __forceinline__ int space_index(float qx, float qy, float qz, float k
   return i;
 }
 
+// Smallest and largest of the wave's lanes.
+__device__ __forceinline__ int wave_min_i32(int x) {
+  x = min(x, __builtin_amdgcn_mov_dpp(x, 0x128, 0xf, 0xf, true));  // row_ror:8, 4, 2, 1
+  x = min(x, __builtin_amdgcn_mov_dpp(x, 0x124, 0xf, 0xf, true));
+  x = min(x, __builtin_amdgcn_mov_dpp(x, 0x122, 0xf, 0xf, true));
+  x = min(x, __builtin_amdgcn_mov_dpp(x, 0x121, 0xf, 0xf, true));
+  return min(min(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+             min(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+}
+__device__ __forceinline__ int wave_max_i32(int x) { return ~wave_min_i32(~x); }
+
+// By order, most tiles of a long sequence lie beyond the last border on one side of all of a wave's
+// rows: one entry for the whole tile then, without a look-up a pair.  -1: a tile that does not.
+struct Span {
+  int lo, hi;  // of the rows' positions
+};
+__device__ __forceinline__ int far_entry(const Span& k, const Span& q, int far) {
+  if (__builtin_elementwise_sub_sat(k.lo, q.hi) >= far) return 2 * far;
+  if (__builtin_elementwise_sub_sat(k.hi, q.lo) <= -far) return 0;
+  return -1;
+}
+
 // Positions of one streamed tile on their way to LDS (order: one array of TK; space: three).
 template <int BIAS, int TK>
 struct StagePos {
@@ -440,9 +475,18 @@ struct StagePos {
                                                tid < 3 * rows ? 4 * tid : kNowhere, 0, 0);
     }
   }
-  __device__ __forceinline__ void store(int* lds, int tid) const {
+  // (order: with the tile's span behind its positions, which end at `rows`)
+  __device__ __forceinline__ void store(int* lds, int rows, int tid) const {
     if constexpr (BIAS == kOrder) {
       if (tid < TK) lds[tid] = (int)v;
+      if (tid < 64) {
+        const bool ok = tid < TK && tid < rows;
+        const int lo = wave_min_i32(ok ? (int)v : INT_MAX), hi = wave_max_i32(ok ? (int)v : INT_MIN);
+        if (tid == 0) {
+          lds[3 * TK] = lo;
+          lds[3 * TK + 1] = hi;
+        }
+      }
     } else if constexpr (BIAS == kSpace) {
       if (tid < 3 * TK) lds[(tid % 3) * TK + tid / 3] = (int)v;
     }
@@ -454,7 +498,7 @@ template <typename T, int DP, int NF>
 struct Tiles {
   static constexpr int TK = kTileOf<T, DP>;
   static constexpr int kOp = TK * Mat<T, DP>::LD;
-  static constexpr size_t kBytes = 2 * kOp * sizeof(T) + (NF + 3) * TK * 4;
+  static constexpr size_t kBytes = 2 * kOp * sizeof(T) + ((NF + 3) * TK + 4) * 4;
   T *a, *b;
   float* f;
   int* pos;
@@ -463,6 +507,9 @@ struct Tiles {
     b = a + kOp;
     f = (float*)(b + kOp);
     pos = (int*)(f + NF * TK);
+  }
+  __device__ __forceinline__ Span span() const {
+    return Span{__builtin_amdgcn_readfirstlane(pos[3 * TK]), __builtin_amdgcn_readfirstlane(pos[3 * TK + 1])};
   }
 };
 
@@ -504,20 +551,6 @@ struct Index {
     }
   }
 };
-
-// A product as an exponent of 2, with its bias and its key's 0 or -inf.  One form for all passes, so
-// that the backward's p are the forward's.
-template <int BIAS>
-__device__ __forceinline__ float score(float x, float c, const float* lut, int i, float off) {
-  if constexpr (BIAS == kNoBias) return fmaf(x, c, off);
-  return fmaf(x, c, lut[i]) + off;
-}
-
-// A float added in LDS without a wait for it.  Only one lane ever adds to an address, so the order of
-// its sum is the lane's own.
-__device__ __forceinline__ void lds_add(float* p, float x) {
-  __hip_atomic_fetch_add(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-}
 
 inline void allow_lds(const void* kernel, size_t bytes) {  // above 64 KB a kernel has to be told
   if (bytes > 65536) (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);

@@ -12,6 +12,13 @@
 namespace hy {
 namespace xa {
 
+// p of a product x, from the forward's lse
+template <bool SCALED, int BIAS>
+__device__ __forceinline__ float power(float x, float c, float bias, float lse) {
+  if constexpr (BIAS == kNoBias) return __builtin_amdgcn_exp2f(SCALED ? x - lse : fmaf(x, c, -lse));
+  return __builtin_amdgcn_exp2f(fmaf(x, c, bias) - lse);
+}
+
 // ------------------------------------------------------------------ query pass
 template <typename T, int DP, int NQ, int BIAS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void bwd_query_kernel(Args a) {
@@ -45,7 +52,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
   typename M::Row qf[NQ], df[NQ];
   Pos qp[NQ];
   f4 dq[NQ][M::DT];
-  float lse[NQ], delta[NQ];
+  float lse[NQ], delta[NQ], c = 1.f;
+  Span span = {INT_MAX, INT_MIN};
   {
     const Rsrc rq = rsrc_of((const T*)a.q + h * a.q_head + (int64_t)tile.start * a.q_row);
     const Rsrc rd = rsrc_of((const T*)a.d_out + h * a.do_head + (int64_t)tile.start * a.do_row);
@@ -57,7 +65,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
       const bool ok = row < rows;
       qf[n] = M::row_global(rq, row * (int)(a.q_row * sizeof(T)), g, a.D, ok, a.unit_q);
       df[n] = M::row_global(rd, row * (int)(a.do_row * sizeof(T)), g, a.D, ok, a.unit_do);
+      c = M::take_scale(qf[n], a.scale);
       qp[n] = load_pos<BIAS>(a.q_pos, tile.start + row, ok);
+      if (BIAS == kOrder) {
+        span.lo = min(span.lo, wave_min_i32(ok ? qp[n].i : INT_MAX));
+        span.hi = max(span.hi, wave_max_i32(ok ? qp[n].i : INT_MIN));
+      }
       // the diagonal of O dO^T, by the very products that give dP: a row with one key has o = v, so its
       // dP - delta is zero and not the rounding of two orders of one sum
       const int at = row * (int)(o_row * sizeof(T));
@@ -83,7 +96,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     }
     for (int i = tid; i < 4 * nb * 64; i += 256) hist[i] = 0.f;
   }
-  const float c = a.scale * kLog2e;
 
   Stage<T, DP> sk, sv;
   typename Stage<T, DP>::Keep keep;
@@ -98,17 +110,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     Stage<T, DP>::keep(keep, a.key_mask, kt, k1 - kt, tid);
     add = tid < k1 - kt && (a.key_mask == nullptr || a.key_mask[kt + (tid & (TK - 1))] != 0) ? 0.f : -INFINITY;
   };
-  auto put = [&](int buf, float flag) {
+  auto put = [&](int buf, int kt, float flag) {
     const L t(smem, buf);
     sk.store(t.a, tid);
     sv.store(t.b, tid);
-    sp.store(t.pos, tid);
+    sp.store(t.pos, k1 - kt, tid);
     if (tid < TK) t.f[tid] = flag;
   };
   if (k0 < k1) {
     masks(k0);
     fetch(k0);
-    put(0, add);
+    put(0, k0, add);
     masks(min(k0 + TK, k1));
   }
   int buf = 0;
@@ -122,6 +134,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     }
     const L t(smem, buf);
     if (active) {
+      const int one = BIAS == kOrder ? far_entry(t.span(), span, a.rule.far) : -1;
+      const float far_bias = one >= 0 ? lut[one] : 0.f;
+      float far_sum = 0.f;
 #pragma unroll
       for (int u = 0; u < TK / 32; ++u) {
         f4 ds[2][NQ];
@@ -133,24 +148,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
           const f4 off = *reinterpret_cast<const f4*>(t.f + at + 4 * g);
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
-            const f4 x = M::dot(kf, qf[n], f4{0.f, 0.f, 0.f, 0.f});
+            const f4 x = M::dot(kf, qf[n], off);
             const f4 dp = M::dot(vf, df[n], f4{0.f, 0.f, 0.f, 0.f});
-            const Index<BIAS, TK> e(t.pos, at + 4 * g, qp[n], a.rule);
+            if (BIAS == kNoBias || one >= 0) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              ds[w][n][r] = __builtin_amdgcn_exp2f(score<BIAS>(x[r], c, lut, e.i[r], off[r]) - lse[n]) *
-                            (dp[r] - delta[n]);
-            if constexpr (BIAS != kNoBias) {
+              for (int r = 0; r < 4; ++r) {
+                ds[w][n][r] = power<M::kScaled, BIAS>(x[r], c, far_bias, lse[n]) * (dp[r] - delta[n]);
+                if (BIAS != kNoBias) far_sum += ds[w][n][r];
+              }
+            } else {
+              const Index<BIAS, TK> e(t.pos, at + 4 * g, qp[n], a.rule);
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                lds_add(hist + (wave * nb + lutb[e.i[r]]) * 64 + lane, ds[w][n][r]);
+              for (int r = 0; r < 4; ++r) {
+                ds[w][n][r] = power<M::kScaled, BIAS>(x[r], c, lut[e.i[r]], lse[n]) * (dp[r] - delta[n]);
+                hist[(wave * nb + lutb[e.i[r]]) * 64 + lane] += ds[w][n][r];
+              }
             }
           }
         }
         M::template outer<NQ, false>(t.a + 32 * u * M::LD, ds[0], ds[1], dq, lane);
       }
+      if (BIAS == kOrder && one >= 0) hist[(wave * nb + lutb[one]) * 64 + lane] += far_sum;
     }
-    if (more) put(buf ^ 1, flag);
+    if (more) put(buf ^ 1, kt + TK, flag);
   }
   if (active) {
 #pragma unroll
@@ -203,7 +223,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
   const bool active = r0 < rows;
   typename M::Row kf[NK], vf[NK];
   Pos kp[NK];
-  float off[NK];
+  float off[NK], c = 1.f;
+  Span span = {INT_MAX, INT_MIN};
   f4 dk[NK][M::DT], dv[NK][M::DT];
   {
     const Rsrc rk = rsrc_of((const T*)a.k + hk * a.k_head + (int64_t)tile.start * a.k_row);
@@ -216,11 +237,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
       vf[n] = M::row_global(rv, row * (int)(a.v_row * sizeof(T)), g, a.D, keep, a.unit_v);
       kp[n] = load_pos<BIAS>(a.k_pos, tile.start + row, ok);
       off[n] = keep ? 0.f : -INFINITY;
+      c = M::take_scale(kf[n], a.scale);  // (the keys' copy, here: the queries' goes into dk)
+      if (BIAS == kOrder) {
+        span.lo = min(span.lo, wave_min_i32(ok ? kp[n].i : INT_MAX));
+        span.hi = max(span.hi, wave_max_i32(ok ? kp[n].i : INT_MIN));
+      }
 #pragma unroll
       for (int d = 0; d < M::DT; ++d) dk[n][d] = dv[n][d] = f4{0.f, 0.f, 0.f, 0.f};
     }
   }
-  const float c = a.scale * kLog2e;
 
   Stage<T, DP> sq, sd;
   typename Stage<T, DP>::Keep all;
@@ -236,11 +261,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     row_lse = ok ? a.lse[at] : INFINITY;
     row_delta = ok ? a.delta[at] : 0.f;
   };
-  auto put = [&](int buf) {
+  auto put = [&](int buf, int qt) {
     const L t(smem, buf);
     sq.store(t.a, tid);
     sd.store(t.b, tid);
-    sp.store(t.pos, tid);
+    sp.store(t.pos, q1 - qt, tid);
     if (tid < TK) {
       t.f[tid] = row_lse;
       t.f[TK + tid] = row_delta;
@@ -249,7 +274,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
   const int per = (q1 - q0 + TK - 1) / TK, steps = per * a.G;  // every query head of the group in turn
   if (steps > 0) {
     fetch(hk * a.G, q0);
-    put(0);
+    put(0, q0);
   }
   for (int i = 0; i < steps; ++i) {
     const int h = hk * a.G + i / per;
@@ -263,6 +288,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     if (more) fetch(hk * a.G + (i + 1) / per, q0 + (i + 1) % per * TK);
     const L t(smem, i & 1);
     if (active) {
+      const int one = BIAS == kOrder ? far_entry(span, t.span(), a.rule.far) : -1;
+      const float far_bias = one >= 0 ? lut[one] : 0.f;
 #pragma unroll
       for (int u = 0; u < TK / 32; ++u) {
         f4 p[2][NK], ds[2][NK];
@@ -275,21 +302,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
           const f4 del = *reinterpret_cast<const f4*>(t.f + TK + at + 4 * g);
 #pragma unroll
           for (int n = 0; n < NK; ++n) {
-            const f4 x = M::dot(qf, kf[n], f4{0.f, 0.f, 0.f, 0.f});
+            const f4 x = M::dot(qf, kf[n], f4(off[n]));
             const f4 dp = M::dot(df, vf[n], f4{0.f, 0.f, 0.f, 0.f});
-            const Index<BIAS, TK, true> e(t.pos, at + 4 * g, kp[n], a.rule);
+            if (BIAS == kNoBias || one >= 0) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              p[w][n][r] = __builtin_amdgcn_exp2f(score<BIAS>(x[r], c, lut, e.i[r], off[n]) - lse[r]);
-              ds[w][n][r] = p[w][n][r] * (dp[r] - del[r]);
+              for (int r = 0; r < 4; ++r) p[w][n][r] = power<M::kScaled, BIAS>(x[r], c, far_bias, lse[r]);
+            } else {
+              const Index<BIAS, TK, true> e(t.pos, at + 4 * g, kp[n], a.rule);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) p[w][n][r] = power<M::kScaled, BIAS>(x[r], c, lut[e.i[r]], lse[r]);
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ds[w][n][r] = p[w][n][r] * (dp[r] - del[r]);
           }
         }
         M::template outer<NK, false>(t.b + 32 * u * M::LD, p[0], p[1], dv, lane);
         M::template outer<NK, false>(t.a + 32 * u * M::LD, ds[0], ds[1], dk, lane);
       }
     }
-    if (more) put((i + 1) & 1);
+    if (more) put((i + 1) & 1, q0 + (i + 1) % per * TK);
   }
   if (!active) return;
 #pragma unroll

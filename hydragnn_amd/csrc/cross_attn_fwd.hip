@@ -29,9 +29,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
 
   const int r0 = wave * 16 * NQ, rows = tile.end - tile.start;  // of the tile
   const bool active = r0 < rows;
-  const float c = fabsf(a.scale) * kLog2e;  // a negative scale turns the queries' signs: the maximum is then
-  typename M::Row qf[NQ];                   // that of the products too
+  typename M::Row qf[NQ];
+  float c = 1.f;
   Pos qp[NQ];
+  Span span = {INT_MAX, INT_MIN};
   f4 o[NQ][M::DT];
   float m[NQ], l[NQ];
   {
@@ -41,8 +42,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
       const int row = r0 + 16 * n + li;
       const bool ok = row < rows;
       qf[n] = M::row_global(rq, row * (int)(a.q_row * sizeof(T)), g, a.D, ok, a.unit_q);
-      if (a.scale < 0.f) M::negate(qf[n]);
+      c = M::take_scale(qf[n], a.scale);
       qp[n] = load_pos<BIAS>(a.q_pos, tile.start + row, ok);
+      if (BIAS == kOrder) {
+        span.lo = min(span.lo, wave_min_i32(ok ? qp[n].i : INT_MAX));
+        span.hi = max(span.hi, wave_max_i32(ok ? qp[n].i : INT_MIN));
+      }
       m[n] = -INFINITY;
       l[n] = 0.f;
 #pragma unroll
@@ -53,6 +58,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     const float* tab = (const float*)a.table + h * a.rule.buckets;
     for (int i = tid; i < lut_size<BIAS>(a.rule); i += 256) lut[i] = tab[lut_bucket<BIAS>(a.rule, i)] * kLog2e;
   }
+
+  // s is an exponent of 2 where the scale or a bias is in it, else a product that c makes one
+  constexpr bool kDone = M::kScaled || BIAS != kNoBias;
+  auto power = [&](float s, float top) {
+    return __builtin_amdgcn_exp2f(kDone ? s - top : fmaf(s, c, -top * c));
+  };
 
   Stage<T, DP> sk, sv;
   typename Stage<T, DP>::Keep keep;
@@ -67,17 +78,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     Stage<T, DP>::keep(keep, a.key_mask, kt, k1 - kt, tid);
     add = tid < k1 - kt && (a.key_mask == nullptr || a.key_mask[kt + (tid & (TK - 1))] != 0) ? 0.f : -INFINITY;
   };
-  auto put = [&](int buf) {
+  auto put = [&](int buf, int kt, float flag) {
     const L t(smem, buf);
     sk.store(t.a, tid);
     sv.store(t.b, tid);
-    sp.store(t.pos, tid);
+    sp.store(t.pos, k1 - kt, tid);
+    if (tid < TK) t.f[tid] = flag;
   };
   if (k0 < k1) {
     masks(k0);
-    if (tid < TK) L(smem, 0).f[tid] = add;
     fetch(k0);
-    put(0);
+    put(0, k0, add);
     masks(min(k0 + TK, k1));
   }
   int buf = 0;
@@ -93,20 +104,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     if (active) {
       f4 s[KB][NQ];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
+      for (int kb = 0; kb < KB; ++kb) {  // a key's 0 or -inf is what its products are added to
         const typename M::Row kf = M::row_lds(t.a + (16 * kb + li) * M::LD, g);
+        const f4 off = *reinterpret_cast<const f4*>(t.f + 16 * kb + 4 * g);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) s[kb][n] = M::dot(kf, qf[n], f4{0.f, 0.f, 0.f, 0.f});
+        for (int n = 0; n < NQ; ++n) s[kb][n] = M::dot(kf, qf[n], off);
       }
+      if constexpr (BIAS != kNoBias) {
+        const int one = BIAS == kOrder ? far_entry(t.span(), span, a.rule.far) : -1;
+        if (one >= 0) {
+          const float b = lut[one];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const int at = 16 * kb + 4 * g;
-        const f4 off = *reinterpret_cast<const f4*>(t.f + at);
+          for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          const Index<BIAS, TK> e(t.pos, at, qp[n], a.rule);
+            for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[kb][n][r] = score<BIAS>(s[kb][n][r], c, lut, e.i[r], off[r]);
+              for (int r = 0; r < 4; ++r) s[kb][n][r] = fmaf(s[kb][n][r], c, b);
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+              const Index<BIAS, TK> e(t.pos, 16 * kb + 4 * g, qp[n], a.rule);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[kb][n][r] = fmaf(s[kb][n][r], c, lut[e.i[r]]);
+            }
         }
       }
       float shrink[NQ];
@@ -119,7 +141,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
           top = fmaxf(fmaxf(fmaxf(fmaxf(top, s[kb][n][0]), s[kb][n][1]), s[kb][n][2]), s[kb][n][3]);
         top = column_max(top);
         const float at = top == -INFINITY ? 0.f : top;  // no key so far: every p is exp2(-inf)
-        shrink[n] = __builtin_amdgcn_exp2f(m[n] - at);
+        shrink[n] = power(m[n], at);
         grown |= top > m[n];
         m[n] = top;
         float sum = 0.f;
@@ -127,7 +149,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            s[kb][n][r] = __builtin_amdgcn_exp2f(s[kb][n][r] - at);
+            s[kb][n][r] = power(s[kb][n][r], at);
             sum += s[kb][n][r];
           }
         // of this lane's keys; the four lanes of a row are joined at the end.  (m = -inf: l is 0.)
@@ -146,10 +168,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
       for (int u = 0; u < TK / 32; ++u)
         M::template outer<NQ, SAVE>(t.b + 32 * u * M::LD, s[2 * u], s[2 * u + 1], o, lane);
     }
-    if (more) {
-      put(buf ^ 1);
-      if (tid < TK) L(smem, buf ^ 1).f[tid] = flag;
-    }
+    if (more) put(buf ^ 1, kt + TK, flag);
   }
   if (!active) return;
 #pragma unroll
@@ -161,7 +180,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
       M::store((T*)a.out + at, o[n], sum > 0.f || sum != sum ? 1.f / sum : 0.f, a.D, g,
                SAVE ? (T*)a.rest + at : nullptr);
       if (SAVE && g == 0)
-        a.lse[(int64_t)h * a.Nq + row] = m[n] == -INFINITY ? INFINITY : m[n] + __builtin_amdgcn_logf(sum);
+        a.lse[(int64_t)h * a.Nq + row] =
+            m[n] == -INFINITY ? INFINITY : (kDone ? m[n] : m[n] * c) + __builtin_amdgcn_logf(sum);
     }
   }
 }
