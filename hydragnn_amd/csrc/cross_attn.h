@@ -71,6 +71,10 @@ struct Args {
   const void* table;  // [H, buckets] fp32
   const void *q_pos, *k_pos;
   Rule rule;
+  // the form for few rows (cross_attn_split.hip): `pack` query heads of a key head and `rows` query rows
+  // a tile, `chunks` times `pack` heads, `split` parts of the keys and their sums
+  int pack, rows, chunks, split;
+  float *part_o, *part_ml;  // [split, Nq, H, D], [split, Nq, H, 2]
   // backward
   const void* d_out;
   int64_t do_row, do_head;
@@ -212,14 +216,21 @@ struct Mat {
       }
     }
   }
+  static __device__ __forceinline__ void spill(float* row, const f4 (&acc)[DT], int g) {  // unrounded
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4*>(row + 16 * dt + 4 * g) = acc[dt];
+  }
   // rounds to T; `rest`, if there is one, takes what the rounding leaves
   static __device__ __forceinline__ void store(T* row, const f4 (&acc)[DT], float mul, int D, int g,
                                                T* rest = nullptr) {
-    typedef typename El<T>::v4 v4;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const int d = 16 * dt + 4 * g;
-      const f4 x = acc[dt] * mul;
+      store4(row, rest, 16 * dt + 4 * g, acc[dt] * mul, D);
+    }
+  }
+  static __device__ __forceinline__ void store4(T* row, T* rest, int d, f4 x, int D) {
+    typedef typename El<T>::v4 v4;
+    {
       const v4 y = __builtin_convertvector(x, v4);
       f4 left = x - __builtin_convertvector(y, f4);
 #pragma unroll
@@ -316,15 +327,19 @@ struct Mat<float, DP> {
         f4 x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = acc[jj * VW + (4 * c + e) % VW][(4 * c + e) / VW] * mul;
-        if ((D & 3) == 0) {
-          if (d < D) *reinterpret_cast<f4*>(row + d) = x;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (d + e < D) row[d + e] = x[e];
-        }
+        store4(row, nullptr, d, x, D);
       }
   }
+  static __device__ __forceinline__ void store4(float* row, float*, int d, f4 x, int D) {
+    if ((D & 3) == 0) {
+      if (d < D) *reinterpret_cast<f4*>(row + d) = x;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d + e < D) row[d + e] = x[e];
+    }
+  }
+  static __device__ __forceinline__ void spill(float* row, const f4 (&acc)[DT], int g) { store(row, acc, 1.f, DP, g); }
 };
 
 // One streamed operand's tile on its way from memory to LDS: 256 threads, 16 bytes

@@ -8,6 +8,8 @@ namespace hy {
 namespace xa {
 
 void forward(const Args& a, at::ScalarType t, int bias, hipStream_t st);
+bool plan_split(Args& a);
+void forward_split(const Args& a, at::ScalarType t, int bias, hipStream_t st);
 void backward(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st);
 int64_t table_tiles(const Args& a, at::ScalarType t, int bias);
 
@@ -23,7 +25,10 @@ static int unit_of(const at::Tensor& t) {
 
 // as it is where its rows can be addressed, else a copy
 static at::Tensor rows(const at::Tensor& t) {
-  return t.dim() == 3 && (t.stride(2) == 1 || t.size(2) <= 1) && t.stride(0) < (1 << 20) ? t : t.contiguous();
+  return t.dim() == 3 && (t.stride(2) == 1 || t.size(2) <= 1) && t.stride(0) < (1 << 20) &&
+                 t.stride(1) < (1 << 20)
+             ? t
+             : t.contiguous();
 }
 
 // rule: [two_sided, side, near, far, thresholds...]
@@ -62,7 +67,8 @@ static int fill(Args& a, const at::Tensor& q, const at::Tensor& k, const at::Ten
   a.unit_q = unit_of(q), a.unit_k = unit_of(k), a.unit_v = unit_of(v);
   // rows of a tile are addressed by 31 bits from its first
   for (const auto& x : {q, k, v})
-    HY_CHECK(x.stride(0) >= 0 && x.stride(0) < (1 << 20) && x.stride(1) >= 0, "cross_attention: row stride");
+    HY_CHECK(x.stride(0) >= 0 && x.stride(0) < (1 << 20) && x.stride(1) >= 0 && x.stride(1) < (1 << 20),
+             "cross_attention: strides");
   a.q_ptr = q_ptr.data_ptr<int>();
   a.k_ptr = k_ptr.data_ptr<int>();
   a.scale = (float)scale;
@@ -122,7 +128,18 @@ static std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_fwd(const at::T
   a.rest = rest.numel() > 0 ? rest.data_ptr() : nullptr;
   a.out = out.data_ptr();
   a.lse = save ? lse.data_ptr<float>() : nullptr;
-  forward(a, q.scalar_type(), bias, stream());
+  if (plan_split(a)) {
+    at::Tensor part;
+    if (a.split > 1) {
+      const int64_t cells = (int64_t)a.split * a.Nq * a.H;
+      part = at::empty({cells * (a.D + 2)}, q.options().dtype(at::kFloat));
+      a.part_o = part.data_ptr<float>();
+      a.part_ml = a.part_o + cells * a.D;
+    }
+    forward_split(a, q.scalar_type(), bias, stream());
+  } else {
+    forward(a, q.scalar_type(), bias, stream());
+  }
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return {out, rest, lse};
 }
@@ -159,7 +176,7 @@ static std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd
   a.d_out = dout.data_ptr();
   a.do_row = dout.stride(0), a.do_head = dout.stride(1);
   a.unit_do = unit_of(dout);
-  HY_CHECK(dout.stride(0) >= 0 && dout.stride(0) < (1 << 20) && dout.stride(1) >= 0, "cross_attention: row stride");
+  HY_CHECK(dout.stride(0) >= 0 && dout.stride(0) < (1 << 20) && dout.stride(1) >= 0, "cross_attention: strides");
   a.unit_o = unit_of(out);
   a.delta = delta.data_ptr<float>();
   a.dq = dq.data_ptr();

@@ -340,7 +340,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
 // the registers.  The key pass holds two accumulators a row and keeps to 16, but for narrow heads.
 static int wave_rows(at::ScalarType t, int bias, int64_t N, int64_t S, int64_t heads) {
   if (t == at::kFloat || bias == kSpace) return 1;
-  return (N / 128 + std::min<int64_t>(S, N)) * heads >= 2 * num_cus() ? 2 : 1;
+  (void)S;
+  return N / 128 * heads >= (bias == kOrder ? 2 : 8) * num_cus() ? 2 : 1;
 }
 
 int64_t table_tiles(const Args& a, at::ScalarType t, int bias) {

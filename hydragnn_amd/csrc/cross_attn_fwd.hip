@@ -198,13 +198,15 @@ static void launch_fwd(const Args& a, hipStream_t st) {
   kern<<<dim3((unsigned)blocks), 256, lds, st>>>(a);
 }
 
-// 16 bits: 32 rows a wave, so that a key fragment read from LDS feeds two products; with distances
-// 16, whose arithmetic wants the registers.
+// 16 bits: 32 rows a wave, so that a key fragment read from LDS feeds two products, where that leaves
+// eight workgroups a compute unit to even out sequences of unlike length; else 16, as with distances,
+// whose arithmetic wants the registers.
 template <typename T, int DP>
 static void pick(const Args& a, int bias, hipStream_t st) {
-  constexpr int NQ = sizeof(T) == 2 ? 2 : 1;
-  if (bias == kNoBias) launch_fwd<T, DP, NQ, kNoBias>(a, st);
-  else if (bias == kOrder) launch_fwd<T, DP, NQ, kOrder>(a, st);
+  constexpr int N2 = sizeof(T) == 2 ? 2 : 1;
+  const bool two = N2 == 2 && (int64_t)(a.Nq / 128) * a.H >= 8 * num_cus();
+  if (bias == kNoBias) two ? launch_fwd<T, DP, N2, kNoBias>(a, st) : launch_fwd<T, DP, 1, kNoBias>(a, st);
+  else if (bias == kOrder) two ? launch_fwd<T, DP, N2, kOrder>(a, st) : launch_fwd<T, DP, 1, kOrder>(a, st);
   else launch_fwd<T, DP, 1, kSpace>(a, st);
 }
 

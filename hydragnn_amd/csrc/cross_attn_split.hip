@@ -1,0 +1,268 @@
+// Ragged cross attention, forward, for few query rows a sequence (one token, a graph's read-out
+// queries) and for few sequences: the keys are split instead of the rows.
+//
+// A workgroup owns one tile of 16 rows, each a query row with one of the heads that share a key head,
+// so that every key and value is read once for all of them.  Its four waves take blocks of 32 keys in
+// turn, a key straight from memory into the product's operand and a value through a piece of LDS that
+// is the wave's own (to be read transposed), without a barrier; they are joined at the end, and so are
+// the `split` workgroups that share a tile's keys, by a second launch.  Bound by the bytes of the keys
+// and values: blocks in flight from many waves, no tile in LDS that a barrier would wait for.
+#include "cross_attn.h"
+
+namespace hy {
+namespace xa {
+
+constexpr int kBlock = 32;  // keys of a wave's step
+
+template <typename T, int DP, int BIAS, bool SAVE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void split_kernel(Args a) {
+  typedef Mat<T, DP> M;
+  constexpr int kPer = El<T>::kPer, CPR = DP / kPer, VC = kBlock * CPR / 64;
+  constexpr int kOwn = kBlock * M::LD;  // of a wave, in elements of T: 16 rows of DP floats fit as well
+  static_assert(kOwn * sizeof(T) >= 16 * DP * 4, "a wave's sums fit its piece of LDS");
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  float* ml = (float*)(smem + 4 * kOwn * sizeof(T));  // [4 waves, 16 rows, 2]
+  float* tab = ml + 128;                              // [pack, buckets]
+  uint8_t* lutb = (uint8_t*)(tab + (BIAS != kNoBias ? a.pack * a.rule.buckets : 0));
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, li = lane & 15;
+  int b = blockIdx.x;
+  const int hk = b % a.Hk;
+  b /= a.Hk;
+  const int h0 = hk * a.G + b % a.chunks * a.pack, heads = min(a.pack, a.G - b % a.chunks * a.pack);
+  b /= a.chunks;
+  const int sp = b % a.split;
+  const Tile tile = find_tile(a.q_ptr, a.S, a.Nq, a.rows, b / a.split);
+  if (tile.start >= tile.end) return;
+  int k0 = 0, k1 = 0;
+  if (tile.seq >= 0) {
+    k0 = min(max(a.k_ptr[tile.seq], 0), a.Nk);
+    k1 = min(max(a.k_ptr[tile.seq + 1], k0), a.Nk);
+  }
+  const T* k = (const T*)a.k + hk * a.k_head;
+  const T* v = (const T*)a.v + hk * a.v_head;
+  T* own = (T*)smem + wave * kOwn;
+
+  const int hl = li % a.pack, qrow = tile.start + li / a.pack;  // this lane's row
+  const bool ok = qrow < tile.end && hl < heads && li / a.pack < a.rows;
+  typename M::Row qf = M::row_global(
+      rsrc_of((const T*)a.q + (int64_t)h0 * a.q_head + (int64_t)tile.start * a.q_row),
+      (qrow - tile.start) * (int)(a.q_row * sizeof(T)) + hl * (int)(a.q_head * sizeof(T)), g, a.D, ok, a.unit_q);
+  const float c = M::take_scale(qf, a.scale);
+  const Pos qp = load_pos<BIAS>(a.q_pos, qrow, ok);
+  if constexpr (BIAS != kNoBias) {
+    for (int i = tid; i < heads * a.rule.buckets; i += 256)
+      tab[i] = ((const float*)a.table)[(int64_t)h0 * a.rule.buckets + i] * kLog2e;
+    for (int i = tid; i < lut_size<BIAS>(a.rule); i += 256) lutb[i] = (uint8_t)lut_bucket<BIAS>(a.rule, i);
+    __syncthreads();
+  }
+  const float* mine = tab + (ok ? hl : 0) * a.rule.buckets;
+  constexpr bool kDone = M::kScaled || BIAS != kNoBias;
+  auto power = [&](float s, float top) {
+    return __builtin_amdgcn_exp2f(kDone ? s - top : fmaf(s, c, -top * c));
+  };
+  auto mask_of = [&](int at) {  // bit i: key at + i takes part
+    bool in = lane < k1 - at && lane < kBlock;
+    if (a.key_mask != nullptr)
+      in = __builtin_amdgcn_raw_buffer_load_b8(rsrc_of(a.key_mask + at), in ? lane : kNowhere, 0, 0) != 0;
+    return (unsigned)__ballot(in);
+  };
+
+  f4 o[1][M::DT];
+#pragma unroll
+  for (int d = 0; d < M::DT; ++d) o[0][d] = f4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  const int step = 4 * a.split * kBlock;
+  int kt = k0 + (sp * 4 + wave) * kBlock;
+  unsigned bits = kt < k1 ? mask_of(kt) : 0;
+  for (; kt < k1; kt += step) {
+    const Rsrc rk = rsrc_of(k + (int64_t)kt * a.k_row), rv = rsrc_of(v + (int64_t)kt * a.v_row);
+    typename M::Row kf[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      kf[t] = M::row_global(rk, (16 * t + li) * (int)(a.k_row * sizeof(T)), g, a.D, bits >> (16 * t + li) & 1, a.unit_k);
+    u4 vr[VC];
+#pragma unroll
+    for (int i = 0; i < VC; ++i) {
+      const int at = lane + 64 * i, row = at / CPR;
+      vr[i] = load16<T>(rv, row * (int)(a.v_row * sizeof(T)), at % CPR * kPer, a.D, bits >> row & 1, a.unit_v);
+    }
+    const unsigned next = kt + step < k1 ? mask_of(kt + step) : 0;
+    f4 s[2][1];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f4 off;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) off[r] = bits >> (16 * t + 4 * g + r) & 1 ? 0.f : -INFINITY;
+      s[t][0] = M::dot(kf[t], qf, off);
+      if constexpr (BIAS != kNoBias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = kt + 16 * t + 4 * g + r;
+          const Pos kp = load_pos<BIAS>(a.k_pos, row, row < k1);
+          const int e = BIAS == kOrder ? order_index(kp.i, qp.i, a.rule.far)
+                                       : space_index(qp.x, qp.y, qp.z, kp.x, kp.y, kp.z, a.rule);
+          s[t][0][r] = fmaf(s[t][0][r], c, mine[lutb[e]]);
+        }
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      top = fmaxf(fmaxf(fmaxf(fmaxf(top, s[t][0][0]), s[t][0][1]), s[t][0][2]), s[t][0][3]);
+    top = column_max(top);
+    const float at = top == -INFINITY ? 0.f : top;
+    const float shrink = power(m, at);
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[t][0][r] = power(s[t][0][r], at);
+        sum += s[t][0][r];
+      }
+    l = fmaf(l, shrink, sum);
+#pragma unroll
+    for (int d = 0; d < M::DT; ++d) o[0][d] *= shrink;
+    m = top;
+    // LDS takes a wave's accesses in order: only the compiler has to keep them so
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < VC; ++i) {
+      const int e = lane + 64 * i;
+      *reinterpret_cast<u4*>(own + (e / CPR) * M::LD + (e % CPR) * kPer) = vr[i];
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    M::template outer<1, SAVE>(own, s[0], s[1], o, lane);
+    asm volatile("" ::: "memory");
+    bits = next;
+  }
+
+  // the waves' sums joined; m as an exponent of 2 from here on
+  l = column_sum(l);
+  if (!kDone) m *= c;
+  __syncthreads();
+  M::spill((float*)own + li * DP, o[0], g);
+  if (g == 0) {
+    ml[(wave * 16 + li) * 2] = m;
+    ml[(wave * 16 + li) * 2 + 1] = l;
+  }
+  __syncthreads();
+  for (int i = tid; i < 16 * DP / 4; i += 256) {
+    const int p = i / (DP / 4), d = i % (DP / 4) * 4, row = tile.start + p / a.pack, h = h0 + p % a.pack;
+    if (row >= tile.end || p % a.pack >= heads || p / a.pack >= a.rows) continue;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[(w * 16 + p) * 2]);
+    f4 x = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float mw = ml[(w * 16 + p) * 2];
+      const float by = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);
+      sum = fmaf(by, ml[(w * 16 + p) * 2 + 1], sum);
+      x += *reinterpret_cast<const f4*>((float*)((T*)smem + w * kOwn) + p * DP + d) * by;
+    }
+    const int64_t cell = (int64_t)row * a.H + h;
+    if (a.split == 1) {
+      M::store4((T*)a.out + cell * a.D, SAVE ? (T*)a.rest + cell * a.D : nullptr, d,
+                x * (sum > 0.f || sum != sum ? 1.f / sum : 0.f), a.D);
+      if (SAVE && d == 0)
+        a.lse[(int64_t)h * a.Nq + row] = top == -INFINITY ? INFINITY : top + __builtin_amdgcn_logf(sum);
+    } else {
+      const int64_t part = (int64_t)sp * a.Nq * a.H + cell;
+      Mat<float, DP>::store4(a.part_o + part * a.D, nullptr, d, x, a.D);
+      if (d == 0) {
+        a.part_ml[2 * part] = top;
+        a.part_ml[2 * part + 1] = sum;
+      }
+    }
+  }
+}
+
+// The splits' sums joined: a thread for four columns of a row and head.
+template <typename T, int DP, bool SAVE>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, cells = (int64_t)a.Nq * a.H, cell = i / (DP / 4);
+  const int d = (int)(i % (DP / 4)) * 4;
+  if (cell >= cells || d >= a.D) return;
+  float top = -INFINITY;
+  for (int s = 0; s < a.split; ++s) top = fmaxf(top, a.part_ml[2 * (s * cells + cell)]);
+  float sum = 0.f;
+  f4 x = f4{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.split; ++s) {
+    const int64_t part = s * cells + cell;
+    const float m = a.part_ml[2 * part];
+    if (m == -INFINITY) continue;  // no key in this part
+    const float by = __builtin_amdgcn_exp2f(m - top);
+    sum = fmaf(by, a.part_ml[2 * part + 1], sum);
+    f4 y;
+    if ((a.D & 3) == 0) {
+      y = *reinterpret_cast<const f4*>(a.part_o + part * a.D + d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = d + e < a.D ? a.part_o[part * a.D + d + e] : 0.f;
+    }
+    x += y * by;
+  }
+  Mat<T, DP>::store4((T*)a.out + cell * a.D, SAVE ? (T*)a.rest + cell * a.D : nullptr, d,
+                     x * (sum > 0.f || sum != sum ? 1.f / sum : 0.f), a.D);
+  if (SAVE && d == 0)
+    a.lse[cell % a.H * a.Nq + cell / a.H] = top == -INFINITY ? INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
+// Whether this form is taken, by sizes alone, and its tiles:
+//   * few rows: on average the rows of a sequence, with the heads that share a key head, fill no more
+//     than one tile of 16.  The form by rows would leave three of its four waves without a row.
+//   * few tiles: the form by rows would not fill the compute units, and there are keys to split.
+// `split` then goes for four workgroups a compute unit, a step of every wave at least.
+bool plan_split(Args& a) {
+  const int64_t S = std::max(a.S, 1), rows = (a.Nq + S - 1) / S, keys = a.Nk / S, cus = num_cus();
+  const bool few = rows * a.G <= 16 || rows <= 2;
+  const int64_t by_rows = (a.Nq / 64 + std::min<int64_t>(a.S, a.Nq)) * a.H;
+  if (!few && !(by_rows < cus && keys >= 4 * kBlock)) return false;
+  a.pack = few ? std::min(a.G, 16) : 1;
+  a.rows = 16 / a.pack;
+  a.chunks = (a.G + a.pack - 1) / a.pack;
+  const int64_t base = (a.Nq / a.rows + std::min<int64_t>(a.S, a.Nq)) * a.chunks * a.Hk;
+  const int64_t most = std::max<int64_t>(keys / (4 * kBlock), 1);
+  a.split = (int)std::max<int64_t>(1, std::min<int64_t>({4 * cus / std::max<int64_t>(base, 1), most, 64}));
+  return true;
+}
+
+template <typename T, int DP, int BIAS, bool SAVE>
+static void launch(const Args& a, hipStream_t st) {
+  const int64_t blocks = tile_count(a.Nq, a.S, a.rows) * a.split * a.chunks * a.Hk;
+  HY_CHECK(blocks < (int64_t(1) << 31), "cross_attention: too many tiles for one launch");
+  size_t lds = 4 * kBlock * Mat<T, DP>::LD * sizeof(T) + 128 * 4;
+  if (BIAS != kNoBias) lds += a.pack * a.rule.buckets * 4 + (BIAS == kOrder ? 2 * a.rule.far + 1 : a.rule.far + 1);
+  auto* kern = &split_kernel<T, DP, BIAS, SAVE>;
+  allow_lds((const void*)kern, lds);
+  kern<<<dim3((unsigned)blocks), 256, lds, st>>>(a);
+  if (a.split > 1)
+    join_kernel<T, DP, SAVE><<<dim3((unsigned)(((int64_t)a.Nq * a.H * (DP / 4) + 255) / 256)), 256, 0, st>>>(a);
+}
+
+template <typename T, int DP>
+static void pick(const Args& a, int bias, hipStream_t st) {
+  const bool save = a.lse != nullptr;
+  if (bias == kNoBias) save ? launch<T, DP, kNoBias, true>(a, st) : launch<T, DP, kNoBias, false>(a, st);
+  else if (bias == kOrder) save ? launch<T, DP, kOrder, true>(a, st) : launch<T, DP, kOrder, false>(a, st);
+  else save ? launch<T, DP, kSpace, true>(a, st) : launch<T, DP, kSpace, false>(a, st);
+}
+
+template <typename T>
+static void pick_width(const Args& a, int bias, hipStream_t st) {
+  if (sizeof(T) == 4 && a.D <= 16) pick<T, sizeof(T) == 4 ? 16 : 32>(a, bias, st);
+  else if (a.D <= 32) pick<T, 32>(a, bias, st);
+  else if (a.D <= 64) pick<T, 64>(a, bias, st);
+  else pick<T, 128>(a, bias, st);
+}
+
+void forward_split(const Args& a, at::ScalarType t, int bias, hipStream_t st) {
+  if (t == at::kFloat) pick_width<float>(a, bias, st);
+  else if (t == at::kBFloat16) pick_width<__bf16>(a, bias, st);
+  else pick_width<_Float16>(a, bias, st);
+}
+
+}  // namespace xa
+}  // namespace hy
