@@ -11,8 +11,8 @@
 // them) and writes y; backward reads x and dy twice and writes dx.  A thread keeps the same 16
 // bytes of channels for all its rows, so the channels' parameters and sums stay in registers.
 //
-// Two forms by size alone (group_norm.hip's `whole`): one workgroup a sequence for short ones (one
-// launch), and chunks of rows whose sums a second launch joins in order for long ones.  Sums of x
+// Two forms by size alone (`whole`): one workgroup a sequence for short ones (one launch), and chunks
+// of rows whose sums a launch between joins in order for long ones.  Sums of x
 // are held in 64 bits, because E[x^2] - E[x]^2 loses what the mean exceeds the deviation by; no sum
 // goes by atomics.
 #include <c10/core/DeviceGuard.h>
@@ -37,6 +37,7 @@ struct Args {
   float* stat;   // [S, G, 2]: mean, inv
   double* part;  // [chunks, G, 2]
   float* cpart;  // [chunks, C, 2]: db, dw of a chunk
+  float* gmean;  // [S, G, 2]: means of w dz and w dz xh
   float *dw, *db;
   int chunks;
 };
@@ -147,6 +148,7 @@ __device__ __forceinline__ void group_sums(int G, int items, Get get, Put put) {
     const int g = g0 + threadIdx.x / P;
     V s0 = 0, s1 = 0;
     if (g < G)
+#pragma unroll 8  // (loads of the chunks' sums in flight together)
       for (int i = sub; i < items; i += P) {
         V t[2];
         get(g, i, t);
@@ -216,46 +218,64 @@ __device__ void zero_rows(T* out, const Rows& r, int C, const Place& p) {
       for (int c = p.tx * PER; c < C; c += p.nx * PER) store<T, PER, VEC>(out + (int64_t)row * C, c, C, z);
 }
 
+// Rows of a thread, `kAhead` at a time so that their loads are in flight together: f(u, row) loads,
+// use(u, row) works on what is there (rows behind the end are loaded again and not used).
+constexpr int kAhead = 4;
+
+template <typename Load, typename Use>
+__device__ __forceinline__ void each_row(const Rows& r, const Place& p, Load load, Use use) {
+  for (int row = r.start + p.ty; row < r.end; row += kAhead * p.ny) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) load(u, min(row + u * p.ny, r.end - 1));
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (row + u * p.ny < r.end) use(u, row + u * p.ny);
+  }
+}
+
+// A thread's sums of PER channels, two of each, on their way to group_sums: [ny][C, 2] in LDS.
+template <typename V, int PER>
+__device__ __forceinline__ void keep_sums(V* red, const Place& p, int c, int C, const V (&s)[PER], const V (&q)[PER]) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (c + i < C) {
+      V* at = red + 2 * ((int64_t)p.ty * C + c + i);
+      at[0] = s[i];
+      at[1] = q[i];
+    }
+}
+
 // ------------------------------------------------------------------ forward
 // Sums of x and x^2 of this workgroup's rows, by group, into put(group, sum, square).
 template <typename T, int PER, bool VEC, typename Put>
 __device__ __forceinline__ void sum_rows(const Args& a, const Rows& r, const Place& p, double* red, Put put) {
-  const int span = p.nx * PER, cg = a.C / a.G;
-  // red: [channels of a block, 2]: the rows' lanes are joined in LDS, channel block by channel block
-  for (int c0 = 0; c0 < a.C; c0 += span) {
-    const int c = c0 + p.tx * PER;
-    double s[PER], q[PER];
+  const int cg = a.C / a.G;
+  if (p.ty < p.ny)
+    for (int c = p.tx * PER; c < a.C; c += p.nx * PER) {
+      double s[PER], q[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = q[i] = 0.0;
-    if (p.ty < p.ny && c < a.C)
-      for (int row = r.start + p.ty; row < r.end; row += p.ny) {
-        float v[PER];
-        load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v);
+      for (int i = 0; i < PER; ++i) s[i] = q[i] = 0.0;
+      float v[kAhead][PER];
+      each_row(
+          r, p,
+          [&](int u, int row) { load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v[u]); },
+          [&](int u, int) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          s[i] += (double)v[i];
-          q[i] = fma((double)v[i], (double)v[i], q[i]);
-        }
-      }
-    // [ny][channels of the block] in turn, summed by channel
-    for (int y = 0; y < p.ny; ++y) {
-      if (p.ty == y && c < a.C) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (c + i < a.C) {
-            double* at = red + 2 * (c0 + p.tx * PER + i);
-            at[0] = (y ? at[0] : 0.0) + s[i];
-            at[1] = (y ? at[1] : 0.0) + q[i];
-          }
-      }
-      __syncthreads();
+            for (int i = 0; i < PER; ++i) {
+              s[i] += (double)v[u][i];
+              q[i] = fma((double)v[u][i], (double)v[u][i], q[i]);
+            }
+          });
+      keep_sums<double, PER>(red, p, c, a.C, s, q);
     }
-  }
+  __syncthreads();
   group_sums<double>(
-      a.G, cg,
+      a.G, cg * p.ny,
       [&](int g, int i, double* t) {
-        t[0] = red[2 * (g * cg + i)];
-        t[1] = red[2 * (g * cg + i) + 1];
+        const int y = i / cg;
+        const double* at = red + 2 * (y * a.C + g * cg + i - y * cg);
+        t[0] = at[0];
+        t[1] = at[1];
       },
       put);
 }
@@ -274,18 +294,19 @@ __device__ __forceinline__ void apply_rows(const Args& a, const Rows& r, const P
       mul[i] = gstat[2 * g + 1] * (a.w != nullptr ? a.w[k] : 1.f);
       add[i] = a.b != nullptr ? a.b[k] : 0.f;
     }
-    for (int row = r.start + p.ty; row < r.end; row += p.ny) {
-      float v[PER];
-      load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v);
+    float v[kAhead][PER];
+    each_row(
+        r, p, [&](int u, int row) { load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v[u]); },
+        [&](int u, int row) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) v[i] = act<ACT>(fmaf(v[i] - mean[i], mul[i], add[i]));
-      store<T, PER, VEC>((T*)a.y + (int64_t)row * a.C, c, a.C, v);
-    }
+          for (int i = 0; i < PER; ++i) v[u][i] = act<ACT>(fmaf(v[u][i] - mean[i], mul[i], add[i]));
+          store<T, PER, VEC>((T*)a.y + (int64_t)row * a.C, c, a.C, v[u]);
+        });
   }
 }
 
-__device__ __forceinline__ void finish_stat(const Args& a, const Rows& r, int g, double s, double q, float* gstat) {
-  const double n = (double)r.length * (double)(a.C / a.G);
+__device__ __forceinline__ void finish_stat(const Args& a, int length, int g, double s, double q, float* gstat) {
+  const double n = (double)length * (double)(a.C / a.G);
   const double mean = s / n, var = q / n - mean * mean;
   const double inv = 1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)a.eps);  // what is no number stays none
   gstat[2 * g] = (float)mean;
@@ -295,13 +316,13 @@ __device__ __forceinline__ void finish_stat(const Args& a, const Rows& r, int g,
 template <typename T, int ACT, bool VEC>
 __global__ __launch_bounds__(kThreads) void fwd_whole_kernel(Args a) {
   constexpr int PER = Vec<T>::kPer;
-  extern __shared__ __attribute__((aligned(16))) double red[];  // [C, 2], then [G, 2] floats
-  float* gstat = (float*)(red + 2 * a.C);
+  extern __shared__ __attribute__((aligned(16))) double red[];  // [ny, C, 2], then [G, 2] floats
   const Rows r = my_rows<true>(a);
   const Place p = place(a.C, PER);
+  float* gstat = (float*)(red + 2 * p.ny * a.C);
   if (r.start >= r.end) return;
   if (r.seq < 0) return zero_rows<T, PER, VEC>((T*)a.y, r, a.C, p);
-  sum_rows<T, PER, VEC>(a, r, p, red, [&](int g, double s, double q) { finish_stat(a, r, g, s, q, gstat); });
+  sum_rows<T, PER, VEC>(a, r, p, red, [&](int g, double s, double q) { finish_stat(a, r.length, g, s, q, gstat); });
   __syncthreads();
   if (a.stat != nullptr)
     for (int i = threadIdx.x; i < 2 * a.G; i += kThreads) a.stat[(int64_t)r.seq * 2 * a.G + i] = gstat[i];
@@ -324,24 +345,11 @@ __global__ __launch_bounds__(kThreads) void fwd_sums_kernel(Args a) {
 template <typename T, int ACT, bool VEC>
 __global__ __launch_bounds__(kThreads) void fwd_apply_kernel(Args a) {
   constexpr int PER = Vec<T>::kPer;
-  extern __shared__ __attribute__((aligned(16))) double red[];
-  float* gstat = (float*)red;
   const Rows r = my_rows<false>(a);
   const Place p = place(a.C, PER);
   if (r.start >= r.end) return;
   if (r.seq < 0) return zero_rows<T, PER, VEC>((T*)a.y, r, a.C, p);
-  const double* from = a.part + (int64_t)r.first * 2 * a.G;
-  group_sums<double>(
-      a.G, r.chunks,
-      [&](int g, int i, double* t) {
-        t[0] = from[((int64_t)i * a.G + g) * 2];
-        t[1] = from[((int64_t)i * a.G + g) * 2 + 1];
-      },
-      [&](int g, double s, double q) { finish_stat(a, r, g, s, q, gstat); });
-  __syncthreads();
-  if (a.stat != nullptr && (int)blockIdx.x == r.first)
-    for (int i = threadIdx.x; i < 2 * a.G; i += kThreads) a.stat[(int64_t)r.seq * 2 * a.G + i] = gstat[i];
-  apply_rows<T, ACT, VEC>(a, r, p, gstat);
+  apply_rows<T, ACT, VEC>(a, r, p, a.stat + (int64_t)r.seq * 2 * a.G);
 }
 
 // ------------------------------------------------------------------ backward
@@ -351,50 +359,47 @@ template <typename T, int ACT, bool VEC, typename Put>
 __device__ __forceinline__ void grad_sums(const Args& a, const Rows& r, const Place& p, float* red, float* cpart,
                                           Put put) {
   constexpr int PER = Vec<T>::kPer;
-  const int span = p.nx * PER, cg = a.C / a.G;
+  const int cg = a.C / a.G;
   const float* stat = a.stat + (int64_t)r.seq * 2 * a.G;
-  for (int c0 = 0; c0 < a.C; c0 += span) {
-    const int c = c0 + p.tx * PER;
-    float s[PER], q[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = q[i] = 0.f;
-    if (p.ty < p.ny && c < a.C) {
-      float mean[PER], inv[PER], w[PER], b[PER];
+  if (p.ty < p.ny)
+    for (int c = p.tx * PER; c < a.C; c += p.nx * PER) {
+      float s[PER], q[PER], mean[PER], inv[PER], w[PER], b[PER];
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int k = min(c + i, a.C - 1), g = k / cg;
+        s[i] = q[i] = 0.f;
         mean[i] = stat[2 * g];
         inv[i] = stat[2 * g + 1];
         w[i] = a.w != nullptr ? a.w[k] : 1.f;
         b[i] = a.b != nullptr ? a.b[k] : 0.f;
       }
-      for (int row = r.start + p.ty; row < r.end; row += p.ny) {
-        float v[PER], d[PER];
-        load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v);
-        load<T, PER, VEC>((const T*)a.dy + (int64_t)row * a.dy_row, c, a.C, d);
+      float v[kAhead][PER], d[kAhead][PER];
+      each_row(
+          r, p,
+          [&](int u, int row) {
+            load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v[u]);
+            load<T, PER, VEC>((const T*)a.dy + (int64_t)row * a.dy_row, c, a.C, d[u]);
+          },
+          [&](int u, int) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const float xh = (v[i] - mean[i]) * inv[i];
-          const float dz = d[i] * act_grad<ACT>(fmaf(xh, w[i], b[i]));
-          s[i] += dz;
-          q[i] = fmaf(dz, xh, q[i]);
-        }
-      }
+            for (int i = 0; i < PER; ++i) {
+              const float xh = (v[u][i] - mean[i]) * inv[i];
+              const float dz = d[u][i] * act_grad<ACT>(fmaf(xh, w[i], b[i]));
+              s[i] += dz;
+              q[i] = fmaf(dz, xh, q[i]);
+            }
+          });
+      keep_sums<float, PER>(red, p, c, a.C, s, q);
     }
-    for (int y = 0; y < p.ny; ++y) {
-      if (p.ty == y && c < a.C) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (c + i < a.C) {
-            float* at = red + 2 * (c + i);
-            at[0] = (y ? at[0] : 0.f) + s[i];
-            at[1] = (y ? at[1] : 0.f) + q[i];
-          }
-      }
-      __syncthreads();
-    }
+  __syncthreads();
+  // by channel, into the first row of `red`; a thread's own channels
+  for (int i = threadIdx.x; i < 2 * a.C; i += kThreads) {
+    float t = red[i];
+    for (int y = 1; y < p.ny; ++y) t += red[2 * y * a.C + i];
+    red[i] = t;
+    cpart[i] = t;
   }
-  for (int i = threadIdx.x; i < 2 * a.C; i += kThreads) cpart[i] = red[i];
+  __syncthreads();
   group_sums<double>(
       a.G, cg,
       [&](int g, int i, double* t) {
@@ -424,18 +429,22 @@ __device__ __forceinline__ void grad_apply(const Args& a, const Rows& r, const P
       m1[i] = gmean[2 * g];
       m2[i] = gmean[2 * g + 1];
     }
-    for (int row = r.start + p.ty; row < r.end; row += p.ny) {
-      float v[PER], d[PER];
-      load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v);
-      load<T, PER, VEC>((const T*)a.dy + (int64_t)row * a.dy_row, c, a.C, d);
+    float v[kAhead][PER], d[kAhead][PER];
+    each_row(
+        r, p,
+        [&](int u, int row) {
+          load<T, PER, VEC>((const T*)a.x + (int64_t)row * a.x_row, c, a.C, v[u]);
+          load<T, PER, VEC>((const T*)a.dy + (int64_t)row * a.dy_row, c, a.C, d[u]);
+        },
+        [&](int u, int row) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const float xh = (v[i] - mean[i]) * inv[i];
-        const float dz = d[i] * act_grad<ACT>(fmaf(xh, w[i], b[i]));
-        v[i] = inv[i] * (product(w[i], dz) - m1[i] - xh * m2[i]);
-      }
-      store<T, PER, VEC>((T*)a.dx + (int64_t)row * a.C, c, a.C, v);
-    }
+          for (int i = 0; i < PER; ++i) {
+            const float xh = (v[u][i] - mean[i]) * inv[i];
+            const float dz = d[u][i] * act_grad<ACT>(fmaf(xh, w[i], b[i]));
+            v[u][i] = inv[i] * (product(w[i], dz) - m1[i] - xh * m2[i]);
+          }
+          store<T, PER, VEC>((T*)a.dx + (int64_t)row * a.C, c, a.C, v[u]);
+        });
   }
 }
 
@@ -443,10 +452,10 @@ template <typename T, int ACT, bool VEC>
 __global__ __launch_bounds__(kThreads) void bwd_whole_kernel(Args a) {
   constexpr int PER = Vec<T>::kPer;
   extern __shared__ __attribute__((aligned(16))) double smem[];
-  float* red = (float*)smem;            // [C, 2]
-  float* gmean = red + 2 * a.C;         // [G, 2]
   const Rows r = my_rows<true>(a);
   const Place p = place(a.C, PER);
+  float* red = (float*)smem;             // [ny, C, 2]
+  float* gmean = red + 2 * p.ny * a.C;   // [G, 2]
   float* cpart = a.cpart + (int64_t)blockIdx.x * 2 * a.C;
   if (r.start >= r.end || r.seq < 0) {
     for (int i = threadIdx.x; i < 2 * a.C; i += kThreads) cpart[i] = 0.f;
@@ -480,35 +489,21 @@ __global__ __launch_bounds__(kThreads) void bwd_sums_kernel(Args a) {
 template <typename T, int ACT, bool VEC>
 __global__ __launch_bounds__(kThreads) void bwd_apply_kernel(Args a) {
   constexpr int PER = Vec<T>::kPer;
-  extern __shared__ __attribute__((aligned(16))) double smem[];
-  float* gmean = (float*)smem;
   const Rows r = my_rows<false>(a);
   const Place p = place(a.C, PER);
   if (r.start >= r.end) return;
   if (r.seq < 0) return zero_rows<T, PER, VEC>((T*)a.dx, r, a.C, p);
-  const double* from = a.part + (int64_t)r.first * 2 * a.G;
-  const double n = (double)r.length * (double)(a.C / a.G);
-  group_sums<double>(
-      a.G, r.chunks,
-      [&](int g, int i, double* t) {
-        t[0] = from[((int64_t)i * a.G + g) * 2];
-        t[1] = from[((int64_t)i * a.G + g) * 2 + 1];
-      },
-      [&](int g, double s, double q) {
-        gmean[2 * g] = (float)(s / n);
-        gmean[2 * g + 1] = (float)(q / n);
-      });
-  __syncthreads();
-  grad_apply<T, ACT, VEC>(a, r, p, gmean);
+  grad_apply<T, ACT, VEC>(a, r, p, a.gmean + (int64_t)r.seq * 2 * a.G);
 }
 
-// dw, db: the chunks' sums of 16 channels a workgroup, 16 threads a channel, in 64 bits and in order
-__global__ __launch_bounds__(256) void bwd_param_kernel(Args a) {
-  __shared__ double sum[16][16][2];
-  const int ch = threadIdx.x & 15, part = threadIdx.x >> 4, c = blockIdx.x * 16 + ch;
+// dw, db: the chunks' sums of 16 channels a workgroup, 64 threads a channel, in 64 bits and in order
+__device__ void param_sums(const Args& a, int block) {
+  __shared__ double sum[64][16][2];
+  const int ch = threadIdx.x & 15, part = threadIdx.x >> 4, c = block * 16 + ch;
   double s = 0.0, q = 0.0;
   if (c < a.C)
-    for (int i = part; i < a.chunks; i += 16) {
+#pragma unroll 4
+    for (int i = part; i < a.chunks; i += 64) {
       const float2 v = *reinterpret_cast<const float2*>(a.cpart + ((int64_t)i * a.C + c) * 2);
       s += v.x;
       q += v.y;
@@ -516,14 +511,64 @@ __global__ __launch_bounds__(256) void bwd_param_kernel(Args a) {
   sum[part][ch][0] = s;
   sum[part][ch][1] = q;
   __syncthreads();
-  if (threadIdx.x < 16 && c < a.C) {
-    for (int i = 1; i < 16; ++i) {
+  if (part < 8) {
+    for (int i = part + 8; i < 64; i += 8) {
+      s += sum[i][ch][0];
+      q += sum[i][ch][1];
+    }
+  }
+  __syncthreads();
+  if (part < 8) {
+    sum[part][ch][0] = s;
+    sum[part][ch][1] = q;
+  }
+  __syncthreads();
+  if (part == 0 && c < a.C) {
+    for (int i = 1; i < 8; ++i) {
       s += sum[i][ch][0];
       q += sum[i][ch][1];
     }
     a.db[c] = (float)s;
     a.dw[c] = (float)q;
   }
+}
+
+// The chunks' sums of 16 groups of a sequence a workgroup, a wave a group: mean and inv (forward), or
+// the means of w dz and w dz xh.  A launch of its own, because every chunk's workgroup would read the
+// sums of all of its sequence's chunks (states of 20000 rows, 320 channels: 39 us with, 25 us without).
+template <bool BACK>
+__device__ void finish_sums(const Args& a, int block) {
+  const int per = (a.G + 15) / 16, seq = block / per, g = block % per * 16 + (threadIdx.x >> 6), lane = lane_id();
+  if (g >= a.G) return;
+  const int s0 = start_of(a, seq + 1), len = max(start_of(a, seq + 2) - s0, 0);
+  if (len == 0) return;
+  const int chunks = (len + a.chunk - 1) / a.chunk;
+  const double* from = a.part + ((int64_t)(s0 / a.chunk + seq + 1) * a.G + g) * 2;
+  double s = 0.0, q = 0.0;
+#pragma unroll 4
+  for (int i = lane; i < chunks; i += 64) {
+    const double2 v = *reinterpret_cast<const double2*>(from + (int64_t)i * a.G * 2);
+    s += v.x;
+    q += v.y;
+  }
+  s = wave_sum(s);
+  q = wave_sum(q);
+  if (lane != 0) return;
+  if constexpr (BACK) {
+    const double n = (double)len * (double)(a.C / a.G);
+    a.gmean[((int64_t)seq * a.G + g) * 2] = (float)(s / n);
+    a.gmean[((int64_t)seq * a.G + g) * 2 + 1] = (float)(q / n);
+  } else {
+    finish_stat(a, len, g, s, q, a.stat + (int64_t)seq * a.G * 2);
+  }
+}
+
+__global__ __launch_bounds__(1024) void fwd_finish_kernel(Args a) { finish_sums<false>(a, blockIdx.x); }
+
+// `finish` workgroups for the means (none where a sequence is one workgroup's), the rest for dw and db
+__global__ __launch_bounds__(1024) void bwd_finish_kernel(Args a, int finish) {
+  if ((int)blockIdx.x < finish) finish_sums<true>(a, blockIdx.x);
+  else param_sums(a, blockIdx.x - finish);
 }
 
 // ------------------------------------------------------------------ host
@@ -550,39 +595,50 @@ static void launch(K* kern, int blocks, size_t lds, hipStream_t st, const Args& 
 
 template <typename T, int ACT, bool VEC>
 static void forward(Args a, hipStream_t st, const at::TensorOptions& opt) {
-  const size_t lds = a.C * 16 + a.G * 8;
+  const int ny = kThreads / std::min((a.C + Vec<T>::kPer - 1) / Vec<T>::kPer, kThreads);
+  const size_t sums = (size_t)ny * a.C * 16, lds = sums + a.G * 8;
   if (whole(a, sizeof(T))) {
     launch(&fwd_whole_kernel<T, ACT, VEC>, a.S + 2, lds, st, a);
     return;
   }
   a.chunk = chunk_rows(a, Vec<T>::kPer);
   a.chunks = (int)tile_count(a.N, a.S, a.chunk);
-  at::Tensor part = at::empty({(int64_t)a.chunks * 2 * a.G}, opt.dtype(at::kDouble));
+  at::Tensor part = at::empty({(int64_t)a.chunks * 2 * a.G}, opt.dtype(at::kDouble)), stat;
   a.part = part.data_ptr<double>();
-  launch(&fwd_sums_kernel<T, VEC>, a.chunks, a.C * 16, st, a);
-  launch(&fwd_apply_kernel<T, ACT, VEC>, a.chunks, a.G * 8, st, a);
+  if (a.stat == nullptr) {
+    stat = at::empty({(int64_t)a.S * 2 * a.G}, opt.dtype(at::kFloat));
+    a.stat = stat.data_ptr<float>();
+  }
+  launch(&fwd_sums_kernel<T, VEC>, a.chunks, sums, st, a);
+  fwd_finish_kernel<<<dim3(a.S * ceil_div(a.G, 16)), 1024, 0, st>>>(a);
+  launch(&fwd_apply_kernel<T, ACT, VEC>, a.chunks, 0, st, a);
 }
 
 template <typename T, int ACT, bool VEC>
 static void backward(Args a, hipStream_t st, const at::TensorOptions& opt) {
-  const size_t lds = a.C * 8 + a.G * 8;
+  const int ny = kThreads / std::min((a.C + Vec<T>::kPer - 1) / Vec<T>::kPer, kThreads);
+  const size_t lds = (size_t)ny * a.C * 8 + a.G * 8;
+  const int params = ceil_div(a.C, 16);
   at::Tensor part, cpart;
   if (whole(a, 2 * sizeof(T))) {
     a.chunks = a.S + 2;
     cpart = at::empty({(int64_t)a.chunks * 2 * a.C}, opt.dtype(at::kFloat));
     a.cpart = cpart.data_ptr<float>();
     launch(&bwd_whole_kernel<T, ACT, VEC>, a.chunks, lds, st, a);
-  } else {
-    a.chunk = chunk_rows(a, Vec<T>::kPer);
-    a.chunks = (int)tile_count(a.N, a.S, a.chunk);
-    part = at::empty({(int64_t)a.chunks * 2 * a.G}, opt.dtype(at::kDouble));
-    cpart = at::empty({(int64_t)a.chunks * 2 * a.C}, opt.dtype(at::kFloat));
-    a.part = part.data_ptr<double>();
-    a.cpart = cpart.data_ptr<float>();
-    launch(&bwd_sums_kernel<T, ACT, VEC>, a.chunks, lds, st, a);
-    launch(&bwd_apply_kernel<T, ACT, VEC>, a.chunks, a.G * 8, st, a);
+    bwd_finish_kernel<<<dim3(params), 1024, 0, st>>>(a, 0);
+    return;
   }
-  bwd_param_kernel<<<dim3(ceil_div(a.C, 16)), 256, 0, st>>>(a);
+  a.chunk = chunk_rows(a, Vec<T>::kPer);
+  a.chunks = (int)tile_count(a.N, a.S, a.chunk);
+  part = at::empty({(int64_t)a.chunks * 2 * a.G}, opt.dtype(at::kDouble));
+  cpart = at::empty({(int64_t)a.chunks * 2 * a.C + (int64_t)a.S * 2 * a.G}, opt.dtype(at::kFloat));
+  a.part = part.data_ptr<double>();
+  a.cpart = cpart.data_ptr<float>();
+  a.gmean = a.cpart + (int64_t)a.chunks * 2 * a.C;
+  launch(&bwd_sums_kernel<T, ACT, VEC>, a.chunks, lds, st, a);
+  const int finish = a.S * ceil_div(a.G, 16);
+  bwd_finish_kernel<<<dim3(finish + params), 1024, 0, st>>>(a, finish);
+  launch(&bwd_apply_kernel<T, ACT, VEC>, a.chunks, 0, st, a);
 }
 
 template <typename T, bool VEC>
