@@ -342,10 +342,11 @@ struct Mat<float, DP> {
   static __device__ __forceinline__ void spill(float* row, const f4 (&acc)[DT], int g) { store(row, acc, 1.f, DP, g); }
 };
 
-// One streamed operand's tile on its way from memory to LDS: 256 threads, 16 bytes
-// each, held in registers while the tile before it is worked on.  Rows behind the sequence and masked
-// ones become zeros, so that whatever they hold (infinities, NaN) meets no product.
-template <typename T, int DP>
+// One streamed operand's tile on its way from memory to LDS: 256 threads, 16 bytes each, held in
+// registers while the tile before it is worked on.  Rows behind the sequence and masked ones become
+// zeros, so that whatever they hold (infinities, NaN) meets no product.  VEC: rows may be read by 16
+// bytes (the loop then has one load a chunk and no branch); else by `unit`.
+template <typename T, int DP, bool VEC>
 struct Stage {
   static constexpr int kPer = El<T>::kPer;
   static constexpr int TK = kTileOf<T, DP>;
@@ -355,6 +356,7 @@ struct Stage {
   struct Keep {  // which of a thread's rows take part
     unsigned m[CH];
   };
+  int at[CH];  // bytes from the tile's first row (VEC: kNowhere behind the width)
   u4 r[CH];
   // base: the tile's first row; rows: how many of it are there
   static __device__ __forceinline__ void keep(Keep& k, const uint8_t* mask, int row0, int rows, int tid) {
@@ -370,13 +372,23 @@ struct Stage {
       k.m[c] = __builtin_amdgcn_raw_buffer_load_b8(r, row < rows ? row : kNowhere, 0, 0);
     }
   }
+  __device__ __forceinline__ void init(int64_t stride, int D, int tid) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = tid + c * 256, d0 = i % CPR * kPer;
+      at[c] = i / CPR * (int)(stride * sizeof(T));
+      if (VEC) at[c] = d0 < D ? at[c] + d0 * (int)sizeof(T) : kNowhere;
+    }
+  }
   __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int rows, const Keep& k, int D, int unit,
                                        int tid) {
     const Rsrc rs = rsrc_of(base + (int64_t)row0 * stride);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int i = tid + c * 256, row = i / CPR;
-      r[c] = load16<T>(rs, row * (int)(stride * sizeof(T)), (i % CPR) * kPer, D, row < rows && k.m[c] != 0, unit);
+      const int i = tid + c * 256;
+      const bool ok = (i / CPR < rows) & (k.m[c] != 0);
+      if constexpr (VEC) r[c] = __builtin_amdgcn_raw_buffer_load_b128(rs, ok ? at[c] : kNowhere, 0, 0);
+      else r[c] = load16<T>(rs, at[c], i % CPR * kPer, D, ok, unit);
     }
   }
   __device__ __forceinline__ void store(T* lds, int tid) const {
@@ -454,6 +466,13 @@ __device__ __forceinline__ int space_index(float qx, float qy, float qz, float k
     i = u < (double)r.far ? (int)u : r.far;
   }
   return i;
+}
+
+// What key `i` of the tile from row0 on adds to its scores: 0, or -inf for one that takes no part.
+__device__ __forceinline__ float key_flag(const uint8_t* mask, int row0, int rows, int i) {
+  const bool in = i < rows;
+  if (mask == nullptr) return in ? 0.f : -INFINITY;
+  return __builtin_amdgcn_raw_buffer_load_b8(rsrc_of(mask + row0), in ? i : kNowhere, 0, 0) != 0 ? 0.f : -INFINITY;
 }
 
 // Smallest and largest of the wave's lanes.

@@ -20,7 +20,7 @@ __device__ __forceinline__ float power(float x, float c, float bias, float lse) 
 }
 
 // ------------------------------------------------------------------ query pass
-template <typename T, int DP, int NQ, int BIAS>
+template <typename T, int DP, int NQ, int BIAS, bool VEC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void bwd_query_kernel(Args a) {
   typedef Mat<T, DP> M;
   typedef Tiles<T, DP, 1> L;
@@ -97,8 +97,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     for (int i = tid; i < 4 * nb * 64; i += 256) hist[i] = 0.f;
   }
 
-  Stage<T, DP> sk, sv;
-  typename Stage<T, DP>::Keep keep;
+  typedef Stage<T, DP, VEC> St;
+  St sk, sv;
+  typename St::Keep keep;
+  sk.init(a.k_row, a.D, tid);
+  sv.init(a.v_row, a.D, tid);
   StagePos<BIAS, TK> sp;
   float add = 0.f;
   auto fetch = [&](int kt) {
@@ -107,8 +110,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     sp.load(a.k_pos, kt, k1 - kt, tid);
   };
   auto masks = [&](int kt) {
-    Stage<T, DP>::keep(keep, a.key_mask, kt, k1 - kt, tid);
-    add = tid < k1 - kt && (a.key_mask == nullptr || a.key_mask[kt + (tid & (TK - 1))] != 0) ? 0.f : -INFINITY;
+    St::keep(keep, a.key_mask, kt, k1 - kt, tid);
+    add = key_flag(a.key_mask, kt, k1 - kt, tid & (TK - 1));
   };
   auto put = [&](int buf, int kt, float flag) {
     const L t(smem, buf);
@@ -202,7 +205,7 @@ __global__ __launch_bounds__(64) void bwd_table_kernel(const float* part, float*
 }
 
 // ------------------------------------------------------------------ key pass
-template <typename T, int DP, int NK, int BIAS>
+template <typename T, int DP, int NK, int BIAS, bool VEC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void bwd_key_kernel(Args a) {
   typedef Mat<T, DP> M;
   typedef Tiles<T, DP, 2> L;
@@ -247,19 +250,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     }
   }
 
-  Stage<T, DP> sq, sd;
-  typename Stage<T, DP>::Keep all;
-  Stage<T, DP>::keep(all, nullptr, 0, 0, tid);
+  typedef Stage<T, DP, VEC> St;
+  St sq, sd;
+  typename St::Keep all;
+  sq.init(a.q_row, a.D, tid);
+  sd.init(a.do_row, a.D, tid);
+  St::keep(all, nullptr, 0, 0, tid);
   StagePos<BIAS, TK> sp;
   float row_lse = INFINITY, row_delta = 0.f;
   auto fetch = [&](int h, int qt) {
     sq.load((const T*)a.q + h * a.q_head, a.q_row, qt, q1 - qt, all, a.D, a.unit_q, tid);
     sd.load((const T*)a.d_out + h * a.do_head, a.do_row, qt, q1 - qt, all, a.D, a.unit_do, tid);
     sp.load(a.q_pos, qt, q1 - qt, tid);
-    const bool ok = tid < TK && tid < q1 - qt;
-    const int64_t at = (int64_t)h * a.Nq + qt + tid;
-    row_lse = ok ? a.lse[at] : INFINITY;
-    row_delta = ok ? a.delta[at] : 0.f;
+    const int64_t at = (int64_t)h * a.Nq + qt;
+    const bool ok = (tid < TK) & (tid < q1 - qt);
+    const int off = ok ? 4 * tid : kNowhere;
+    const unsigned lse = __builtin_amdgcn_raw_buffer_load_b32(rsrc_of(a.lse + at), off, 0, 0);
+    row_lse = ok ? __uint_as_float(lse) : INFINITY;  // exp2(z - inf): a row that is not there has no p
+    row_delta = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc_of(a.delta + at), off, 0, 0));
   };
   auto put = [&](int buf, int qt) {
     const L t(smem, buf);
@@ -355,7 +363,8 @@ static void launch_query(const Args& a, float* dtable, hipStream_t st) {
   HY_CHECK(qt * a.H < (int64_t(1) << 31), "cross_attention: too many tiles for one launch");
   size_t lds = 2 * Tiles<T, DP, 1>::kBytes;
   if (BIAS != kNoBias) lds += 4 * a.rule.buckets * 64 * 4 + nl * 5;
-  auto* kern = &bwd_query_kernel<T, DP, NQ, BIAS>;
+  auto* kern = a.unit_k == 16 && a.unit_v == 16 ? &bwd_query_kernel<T, DP, NQ, BIAS, true>
+                                                : &bwd_query_kernel<T, DP, NQ, BIAS, false>;
   allow_lds((const void*)kern, lds);
   kern<<<dim3((unsigned)(qt * a.H)), 256, lds, st>>>(a);
   if (BIAS != kNoBias) {
@@ -370,7 +379,8 @@ static void launch_key(const Args& a, hipStream_t st) {
   const int64_t kt = tile_count(a.Nk, a.S, 64 * NK);
   HY_CHECK(kt * a.Hk < (int64_t(1) << 31), "cross_attention: too many tiles for one launch");
   const size_t lds = 2 * Tiles<T, DP, 2>::kBytes + nl * 4;
-  auto* kern = &bwd_key_kernel<T, DP, NK, BIAS>;
+  auto* kern = a.unit_q == 16 && a.unit_do == 16 ? &bwd_key_kernel<T, DP, NK, BIAS, true>
+                                                 : &bwd_key_kernel<T, DP, NK, BIAS, false>;
   allow_lds((const void*)kern, lds);
   kern<<<dim3((unsigned)(kt * a.Hk)), 256, lds, st>>>(a);
 }

@@ -7,7 +7,7 @@
 namespace hy {
 namespace xa {
 
-template <typename T, int DP, int NQ, int BIAS, bool SAVE>
+template <typename T, int DP, int NQ, int BIAS, bool SAVE, bool VEC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void fwd_kernel(Args a) {
   typedef Mat<T, DP> M;
   typedef Tiles<T, DP, 1> L;
@@ -65,8 +65,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     return __builtin_amdgcn_exp2f(kDone ? s - top : fmaf(s, c, -top * c));
   };
 
-  Stage<T, DP> sk, sv;
-  typename Stage<T, DP>::Keep keep;
+  typedef Stage<T, DP, VEC> St;
+  St sk, sv;
+  typename St::Keep keep;
+  sk.init(a.k_row, a.D, tid);
+  sv.init(a.v_row, a.D, tid);
   StagePos<BIAS, TK> sp;
   auto fetch = [&](int kt) {  // a tile's rows, with the masks that the call before has fetched
     sk.load(k, a.k_row, kt, k1 - kt, keep, a.D, a.unit_k, tid);
@@ -75,8 +78,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
   };
   float add = 0.f;
   auto masks = [&](int kt) {
-    Stage<T, DP>::keep(keep, a.key_mask, kt, k1 - kt, tid);
-    add = tid < k1 - kt && (a.key_mask == nullptr || a.key_mask[kt + (tid & (TK - 1))] != 0) ? 0.f : -INFINITY;
+    St::keep(keep, a.key_mask, kt, k1 - kt, tid);
+    add = key_flag(a.key_mask, kt, k1 - kt, tid & (TK - 1));
   };
   auto put = [&](int buf, int kt, float flag) {
     const L t(smem, buf);
@@ -193,7 +196,10 @@ static void launch_fwd(const Args& a, hipStream_t st) {
   size_t lds = 2 * Tiles<T, DP, 1>::kBytes;
   if (BIAS == kOrder) lds += (2 * a.rule.far + 1) * 4;
   if (BIAS == kSpace) lds += (a.rule.far + 1) * 4;
-  auto* kern = a.lse != nullptr ? &fwd_kernel<T, DP, NQ, BIAS, true> : &fwd_kernel<T, DP, NQ, BIAS, false>;
+  const bool vec = a.unit_k == 16 && a.unit_v == 16;
+  auto* kern = a.lse != nullptr
+                   ? (vec ? &fwd_kernel<T, DP, NQ, BIAS, true, true> : &fwd_kernel<T, DP, NQ, BIAS, true, false>)
+                   : (vec ? &fwd_kernel<T, DP, NQ, BIAS, false, true> : &fwd_kernel<T, DP, NQ, BIAS, false, false>);
   allow_lds((const void*)kern, lds);
   kern<<<dim3((unsigned)blocks), 256, lds, st>>>(a);
 }
