@@ -451,19 +451,21 @@ __device__ __forceinline__ int order_index(int kp, int qp, int far) {
   return i + far;
 }
 
-// Entry of a pair by distance: floor(dist / unit).  In fp32 first; where that lies within its own
-// rounding (2^-20 relative covers the difference, the squares, the root and 1 / unit) of a whole
-// number, again in 64 bits, so that the bucket is the one that 64 bits give, on a lattice too.
+// Entry of a pair by distance: the largest whole n with (n unit)^2 <= distance^2.  In fp32 first;
+// where that lies within its own rounding (2^-20 relative covers the difference, the squares, the root
+// and 1 / unit) of a whole number, by that comparison in 64 bits, in which fp32 coordinates' squares
+// and their sum are as good as exact: the bucket is the true one, on a lattice too.
 __device__ __forceinline__ int space_index(float qx, float qy, float qz, float kx, float ky, float kz, const Rule& r) {
   const float dx = kx - qx, dy = ky - qy, dz = kz - qz;
   const float t = __builtin_amdgcn_sqrtf(fmaf(dx, dx, fmaf(dy, dy, dz * dz))) * r.inv_unit;
-  const float far = (float)r.far;
+  const float far = (float)r.far, near = rintf(t);
   int i = t < far ? (int)t : r.far;  // not a number: far
-  if (fabsf(t - rintf(t)) < t * 0x1p-20f && t < far + 1.f) {
+  if (fabsf(t - near) < t * 0x1p-20f && t < far + 1.f) {
 #pragma clang fp contract(off)
     const double ex = (double)kx - (double)qx, ey = (double)ky - (double)qy, ez = (double)kz - (double)qz;
-    const double u = __builtin_sqrt(ex * ex + ey * ey + ez * ez) / r.unit;
-    i = u < (double)r.far ? (int)u : r.far;
+    const double border = (double)near * r.unit;
+    i = (int)near - (ex * ex + ey * ey + ez * ez >= border * border ? 0 : 1);
+    i = min(i, r.far);
   }
   return i;
 }

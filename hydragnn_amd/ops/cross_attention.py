@@ -53,9 +53,9 @@ class RelativeBuckets:
     * ``unit=None``: positions are whole numbers (int32 [rows], the order of a sequence), n is
       |k_pos - q_pos|.  ``bidirectional``: keys behind the query have the second half of the
       ``num_buckets``; otherwise they all count as distance 0.
-    * ``unit=u``: positions are points (fp32 [rows, 3]), n is floor(distance / u), exact to the
-      border (64-bit arithmetic where 32 bits leave a doubt).  A distance that is not a number
-      counts as far.
+    * ``unit=u``: positions are points (fp32 [rows, 3]), n is the largest whole number with
+      (n u)^2 <= distance^2, compared in 64 bits wherever 32 leave a doubt.  A distance that is not
+      a number counts as far.
 
     >>> RelativeBuckets(32, 128)             # orders, both directions
     >>> RelativeBuckets(32, 64, unit=0.25)   # distances: steps of 0.25 up to 4, then wider, far from 16 on
@@ -88,8 +88,9 @@ class RelativeBuckets:
         first = 0
         if self.unit is not None:
             d = k_pos.double().unsqueeze(-3) - q_pos.double().unsqueeze(-2)
-            d = torch.sqrt(d[..., 0] * d[..., 0] + d[..., 1] * d[..., 1] + d[..., 2] * d[..., 2]) / self.unit
-            n = torch.where(d < self.max_distance, d, torch.full_like(d, self.max_distance)).long()
+            d = d[..., 0] * d[..., 0] + d[..., 1] * d[..., 1] + d[..., 2] * d[..., 2]
+            borders = torch.arange(1, self.max_distance + 1, dtype=d.dtype, device=d.device) * self.unit
+            n = torch.bucketize(d, borders * borders, right=True)  # (not a number: behind the last)
         else:
             rel = k_pos.long().unsqueeze(-2) - q_pos.long().unsqueeze(-1)
             if self.bidirectional:
