@@ -342,17 +342,17 @@ struct Mat<float, DP> {
   static __device__ __forceinline__ void spill(float* row, const f4 (&acc)[DT], int g) { store(row, acc, 1.f, DP, g); }
 };
 
-// One streamed operand's tile on its way from memory to LDS: 256 threads, 16 bytes each, held in
+// One streamed operand's tile on its way from memory to LDS: NT threads, 16 bytes each, held in
 // registers while the tile before it is worked on.  Rows behind the sequence and masked ones become
 // zeros, so that whatever they hold (infinities, NaN) meets no product.  VEC: rows may be read by 16
 // bytes (the loop then has one load a chunk and no branch); else by `unit`.
-template <typename T, int DP, bool VEC>
+template <typename T, int DP, bool VEC, int NT>
 struct Stage {
   static constexpr int kPer = El<T>::kPer;
   static constexpr int TK = kTileOf<T, DP>;
-  static constexpr int CPR = DP / kPer;      // 16-byte chunks of a row
-  static constexpr int CH = TK * CPR / 256;  // of one thread
-  static_assert(TK * CPR % 256 == 0, "a tile is a whole number of chunks a thread");
+  static constexpr int CPR = DP / kPer;     // 16-byte chunks of a row
+  static constexpr int CH = TK * CPR / NT;  // of one thread
+  static_assert(TK * CPR % NT == 0, "a tile is a whole number of chunks a thread");
   struct Keep {  // which of a thread's rows take part
     unsigned m[CH];
   };
@@ -368,14 +368,14 @@ struct Stage {
     const Rsrc r = rsrc_of(mask + row0);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int row = (tid + c * 256) / CPR;
+      const int row = (tid + c * NT) / CPR;
       k.m[c] = __builtin_amdgcn_raw_buffer_load_b8(r, row < rows ? row : kNowhere, 0, 0);
     }
   }
   __device__ __forceinline__ void init(int64_t stride, int D, int tid) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int i = tid + c * 256, d0 = i % CPR * kPer;
+      const int i = tid + c * NT, d0 = i % CPR * kPer;
       at[c] = i / CPR * (int)(stride * sizeof(T));
       if (VEC) at[c] = d0 < D ? at[c] + d0 * (int)sizeof(T) : kNowhere;
     }
@@ -385,7 +385,7 @@ struct Stage {
     const Rsrc rs = rsrc_of(base + (int64_t)row0 * stride);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int i = tid + c * 256;
+      const int i = tid + c * NT;
       const bool ok = (i / CPR < rows) & (k.m[c] != 0);
       if constexpr (VEC) r[c] = __builtin_amdgcn_raw_buffer_load_b128(rs, ok ? at[c] : kNowhere, 0, 0);
       else r[c] = load16<T>(rs, at[c], i % CPR * kPer, D, ok, unit);
@@ -394,7 +394,7 @@ struct Stage {
   __device__ __forceinline__ void store(T* lds, int tid) const {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int i = tid + c * 256;
+      const int i = tid + c * NT;
       *reinterpret_cast<u4*>(lds + (i / CPR) * Mat<T, DP>::LD + (i % CPR) * kPer) = r[c];
     }
   }
@@ -500,31 +500,38 @@ __device__ __forceinline__ int far_entry(const Span& k, const Span& q, int far) 
 }
 
 // Positions of one streamed tile on their way to LDS (order: one array of TK; space: three).
-template <int BIAS, int TK>
+template <int BIAS, int TK, int NT>
 struct StagePos {
-  unsigned v;
+  static constexpr int kN = BIAS == kSpace ? 3 * TK : TK, PC = (kN + NT - 1) / NT;
+  unsigned v[PC];
   __device__ __forceinline__ void load(const void* pos, int row0, int rows, int tid) {
-    if constexpr (BIAS == kOrder) {
-      v = __builtin_amdgcn_raw_buffer_load_b32(rsrc_of((const int*)pos + row0), tid < rows ? 4 * tid : kNowhere, 0, 0);
-    } else if constexpr (BIAS == kSpace) {
-      v = __builtin_amdgcn_raw_buffer_load_b32(rsrc_of((const float*)pos + (int64_t)row0 * 3),
-                                               tid < 3 * rows ? 4 * tid : kNowhere, 0, 0);
+    if constexpr (BIAS == kNoBias) return;
+    constexpr int kPerRow = BIAS == kSpace ? 3 : 1;
+    const Rsrc r = rsrc_of((const int*)pos + (int64_t)row0 * kPerRow);
+#pragma unroll
+    for (int c = 0; c < PC; ++c) {
+      const int i = tid + c * NT;
+      v[c] = __builtin_amdgcn_raw_buffer_load_b32(r, (i < kN) & (i < kPerRow * rows) ? 4 * i : kNowhere, 0, 0);
     }
   }
   // (order: with the tile's span behind its positions, which end at `rows`)
   __device__ __forceinline__ void store(int* lds, int rows, int tid) const {
     if constexpr (BIAS == kOrder) {
-      if (tid < TK) lds[tid] = (int)v;
+      if (tid < TK) lds[tid] = (int)v[0];
       if (tid < 64) {
         const bool ok = tid < TK && tid < rows;
-        const int lo = wave_min_i32(ok ? (int)v : INT_MAX), hi = wave_max_i32(ok ? (int)v : INT_MIN);
+        const int lo = wave_min_i32(ok ? (int)v[0] : INT_MAX), hi = wave_max_i32(ok ? (int)v[0] : INT_MIN);
         if (tid == 0) {
           lds[3 * TK] = lo;
           lds[3 * TK + 1] = hi;
         }
       }
     } else if constexpr (BIAS == kSpace) {
-      if (tid < 3 * TK) lds[(tid % 3) * TK + tid / 3] = (int)v;
+#pragma unroll
+      for (int c = 0; c < PC; ++c) {
+        const int i = tid + c * NT;
+        if (i < kN) lds[i % 3 * TK + i / 3] = (int)v[c];
+      }
     }
   }
 };
@@ -587,6 +594,87 @@ struct Index {
     }
   }
 };
+
+// The four waves of a workgroup: RW of them own rows, and KS groups of those take the streamed tiles
+// in turn, each with its own buffers; the groups' sums are joined in LDS at the end.
+//   RW 4, KS 1: every tile in LDS serves four waves.
+//   RW 2, KS 2: twice the workgroups, of half the length.  For a launch that leaves few of them to a
+//               compute unit, where the longest sequence's workgroup is what it waits for.
+// A wave's accumulators as they lie in registers, [N][DT] of 64 lanes:
+template <int N, int DT>
+__device__ __forceinline__ void put_acc(float* at, const f4 (&acc)[N][DT], int lane) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f4*>(at + ((n * DT + d) * 64 + lane) * 4) = acc[n][d];
+}
+template <int N, int DT>
+__device__ __forceinline__ void add_acc(const float* at, f4 (&acc)[N][DT], int lane) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[n][d] += *reinterpret_cast<const f4*>(at + ((n * DT + d) * 64 + lane) * 4);
+}
+
+// 16 `per` rows a wave and `waves` of them that own rows: a workgroup's rows
+struct Form {
+  int per, waves;
+  int rows() const { return 16 * per * waves; }
+};
+inline int lut_entries(const Args& a, int bias) {
+  return bias == kOrder ? 2 * a.rule.far + 1 : bias == kSpace ? a.rule.far + 1 : 0;
+}
+inline size_t table_bytes(const Args& a, int bias, bool sums) {  // of LDS: the look-up table, and the gradient's sums
+  return (size_t)lut_entries(a, bias) * (sums ? 5 : 4) + (sums && bias != kNoBias ? 4 * a.rule.buckets * 64 * 4 : 0);
+}
+// RW 2, KS 2 for fewer than four workgroups of 64 rows a compute unit (two in 16 bits, whose products
+// are short beside the tiles' way through LDS), if two of them fit its LDS.  8 sequences of up to 512 on
+// 777 rows, 8 heads of 64, float: 38 us with, 54 us without; the key pass of 8 of up to 1024 on 2048
+// rows, 4 key heads of 64, bfloat16: 105 us and 99 us.  The query pass with a bias keeps to RW 4: its
+// sums fill LDS (32 graphs of up to 126 atoms, 8 heads of 8, float, distances: 25 us and 19 us).
+template <int NF>
+bool few_workgroups(int64_t N, int64_t S, int64_t heads, at::ScalarType t, int64_t D, size_t more) {
+  size_t b;  // of one buffer
+  if (t == at::kFloat)
+    b = D <= 16   ? Tiles<float, 16, NF>::kBytes
+        : D <= 32 ? Tiles<float, 32, NF>::kBytes
+        : D <= 64 ? Tiles<float, 64, NF>::kBytes
+                  : Tiles<float, 128, NF>::kBytes;
+  else
+    b = D <= 32   ? Tiles<__bf16, 32, NF>::kBytes
+        : D <= 64 ? Tiles<__bf16, 64, NF>::kBytes
+                  : Tiles<__bf16, 128, NF>::kBytes;
+  return (N / 64 + std::min(S, N)) * heads < (t == at::kFloat ? 4 : 2) * num_cus() && 4 * b + more <= 80 * 1024;
+}
+
+// The query pass: 32 rows a wave in 16 bits, so that a fragment read from LDS feeds two products, from
+// eight workgroups a compute unit on that even out sequences of unlike length (8 sequences of up to
+// 1024 on 2048 rows, 16 heads of 64, forward: 52 us with 16 rows, 62 us with 32); by order from two (its
+// table of sums in LDS goes by waves); 16 with distances, whose arithmetic wants the registers,
+// and with rows that are not aligned.
+inline Form query_form(const Args& a, at::ScalarType t, int bias) {
+  if (bias == kNoBias && few_workgroups<1>(a.Nq, a.S, a.H, t, a.D, 0)) return Form{1, 2};
+  if (t == at::kFloat || bias == kSpace || a.unit_k != 16 || a.unit_v != 16) return Form{1, 4};
+  return Form{(int64_t)(a.Nq / 128) * a.H >= (bias == kOrder ? 2 : 8) * num_cus() ? 2 : 1, 4};
+}
+
+// The forward pass, as the query pass but for the table of sums.
+inline Form forward_form(const Args& a, at::ScalarType t, int bias) {
+  if (few_workgroups<1>(a.Nq, a.S, a.H, t, a.D, table_bytes(a, bias, false))) return Form{1, 2};
+  if (t == at::kFloat || bias == kSpace || a.unit_k != 16 || a.unit_v != 16) return Form{1, 4};
+  return Form{(int64_t)(a.Nq / 128) * a.H >= 8 * num_cus() ? 2 : 1, 4};
+}
+
+// The key pass holds two accumulators a row and keeps to 16 rows a wave, but for narrow heads.
+inline Form key_form(const Args& a, at::ScalarType t, int bias) {
+  if (few_workgroups<2>(a.Nk, a.S, a.Hk, t, a.D, table_bytes(a, bias, false))) return Form{1, 2};
+  if (t == at::kFloat || bias == kSpace || a.D > 32 || a.unit_q != 16 || a.unit_do != 16) return Form{1, 4};
+  return Form{(int64_t)(a.Nk / 128) * a.Hk >= 8 * num_cus() ? 2 : 1, 4};
+}
+
+inline int64_t table_tiles(const Args& a, at::ScalarType t, int bias) {
+  return tile_count(a.Nq, a.S, query_form(a, t, bias).rows());
+}
 
 inline void allow_lds(const void* kernel, size_t bytes) {  // above 64 KB a kernel has to be told
   if (bytes > 65536) (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);

@@ -7,11 +7,12 @@
 namespace hy {
 namespace xa {
 
-void forward(const Args& a, at::ScalarType t, int bias, hipStream_t st);
+template <typename T>
+void forward_rows(const Args& a, at::ScalarType t, int bias, hipStream_t st);
+template <typename T>
+void backward_rows(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st);
 bool plan_split(Args& a);
 void forward_split(const Args& a, at::ScalarType t, int bias, hipStream_t st);
-void backward(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st);
-int64_t table_tiles(const Args& a, at::ScalarType t, int bias);
 
 typedef c10::optional<at::Tensor> OptTensor;
 
@@ -138,7 +139,10 @@ static std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_fwd(const at::T
     }
     forward_split(a, q.scalar_type(), bias, stream());
   } else {
-    forward(a, q.scalar_type(), bias, stream());
+    const auto t = q.scalar_type();
+    if (t == at::kFloat) forward_rows<float>(a, t, bias, stream());
+    else if (t == at::kBFloat16) forward_rows<__bf16>(a, t, bias, stream());
+    else forward_rows<_Float16>(a, t, bias, stream());
   }
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return {out, rest, lse};
@@ -183,7 +187,11 @@ static std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd
   a.dk = dk.data_ptr();
   a.dv = dv.data_ptr();
   a.part = bias != kNoBias ? part.data_ptr<float>() : nullptr;
-  backward(a, q.scalar_type(), bias, bias != kNoBias ? dtable.data_ptr<float>() : nullptr, stream());
+  const auto t = q.scalar_type();
+  float* dt = bias != kNoBias ? dtable.data_ptr<float>() : nullptr;
+  if (t == at::kFloat) backward_rows<float>(a, t, bias, dt, stream());
+  else if (t == at::kBFloat16) backward_rows<__bf16>(a, t, bias, dt, stream());
+  else backward_rows<_Float16>(a, t, bias, dt, stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return {dq, dk, dv, dtable};
 }

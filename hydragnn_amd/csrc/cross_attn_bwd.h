@@ -7,6 +7,8 @@
 // the same bits: the query pass (dq, delta, the table's sums), whose waves own 16 query rows each and
 // stream the keys, and the key pass (dk, dv), whose waves own 16 keys each and stream the queries of
 // every head that shares them.
+#pragma once
+
 #include "cross_attn.h"
 
 namespace hy {
@@ -20,23 +22,25 @@ __device__ __forceinline__ float power(float x, float c, float bias, float lse) 
 }
 
 // ------------------------------------------------------------------ query pass
-template <typename T, int DP, int NQ, int BIAS, bool VEC>
+template <typename T, int DP, int NQ, int BIAS, bool VEC, int RW, int KS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void bwd_query_kernel(Args a) {
   typedef Mat<T, DP> M;
   typedef Tiles<T, DP, 1> L;
-  constexpr int ROWS = 64 * NQ, TK = L::TK;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  float* hist = (float*)(smem + 2 * L::kBytes);  // [4 waves, buckets, 64 lanes]: every lane adds to its own column
+  constexpr int ROWS = 16 * NQ * RW, NT = 64 * RW, TK = L::TK;
+  extern __shared__ __attribute__((aligned(16))) uint8_t shared[];
+  float* hist = (float*)(shared + KS * 2 * L::kBytes);  // [4 waves, buckets, 64 lanes]: a lane adds to its own column
   const int nb = BIAS != kNoBias ? a.rule.buckets : 0;
   float* lut = hist + 4 * nb * 64;
   const int nl = BIAS != kNoBias ? lut_size<BIAS>(a.rule) : 0;
   uint8_t* lutb = (uint8_t*)(lut + nl);
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, li = lane & 15;
+  const int tid = threadIdx.x % NT, lane = tid & 63, wave = tid >> 6, g = lane >> 4, li = lane & 15;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  uint8_t* smem = shared + group * 2 * L::kBytes;
   const int h = blockIdx.x % a.H;
   const Tile tile = find_tile(a.q_ptr, a.S, a.Nq, ROWS, blockIdx.x / a.H);
   if (tile.start >= tile.end) {
-    if (BIAS != kNoBias && tid < nb) a.part[(int64_t)blockIdx.x * nb + tid] = 0.f;
+    if (BIAS != kNoBias && (int)threadIdx.x < nb) a.part[(int64_t)blockIdx.x * nb + threadIdx.x] = 0.f;
     return;
   }
   int k0 = 0, k1 = 0;
@@ -82,27 +86,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
       delta[n] = column_sum(mine);
       const int64_t to = (int64_t)h * a.Nq + tile.start + row;
       lse[n] = ok ? a.lse[to] : INFINITY;  // exp2(z - inf): a row that is not there has no p
-      if (ok && g == 0) a.delta[to] = delta[n];
+      if (ok && g == 0 && group == 0) a.delta[to] = delta[n];
 #pragma unroll
       for (int d = 0; d < M::DT; ++d) dq[n][d] = f4{0.f, 0.f, 0.f, 0.f};
     }
   }
   if constexpr (BIAS != kNoBias) {
     const float* tab = (const float*)a.table + h * nb;
-    for (int i = tid; i < nl; i += 256) {
+    for (int i = threadIdx.x; i < nl; i += 256) {
       const int b = lut_bucket<BIAS>(a.rule, i);
       lut[i] = tab[b] * kLog2e;
       lutb[i] = (uint8_t)b;
     }
-    for (int i = tid; i < 4 * nb * 64; i += 256) hist[i] = 0.f;
+    for (int i = threadIdx.x; i < 4 * nb * 64; i += 256) hist[i] = 0.f;
   }
 
-  typedef Stage<T, DP, VEC> St;
+  typedef Stage<T, DP, VEC, NT> St;
   St sk, sv;
   typename St::Keep keep;
   sk.init(a.k_row, a.D, tid);
   sv.init(a.v_row, a.D, tid);
-  StagePos<BIAS, TK> sp;
+  StagePos<BIAS, TK, NT> sp;
   float add = 0.f;
   auto fetch = [&](int kt) {
     sk.load(k, a.k_row, kt, k1 - kt, keep, a.D, a.unit_k, tid);
@@ -120,23 +124,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     sp.store(t.pos, k1 - kt, tid);
     if (tid < TK) t.f[tid] = flag;
   };
-  if (k0 < k1) {
-    masks(k0);
-    fetch(k0);
-    put(0, k0, add);
-    masks(min(k0 + TK, k1));
+  float* own = hist + (group * RW + wave) * nb * 64 + lane;
+  constexpr int kStep = KS * TK;
+  int kt = k0 + group * TK;  // (a group may have a tile less than the first)
+  if (kt < k1) {
+    masks(kt);
+    fetch(kt);
+    put(0, kt, add);
+    masks(min(kt + kStep, k1));
   }
   int buf = 0;
-  for (int kt = k0; kt < k1; kt += TK, buf ^= 1) {
+  for (int first = k0; first < k1; first += kStep, kt += kStep, buf ^= 1) {
     __syncthreads();
-    const bool more = kt + TK < k1;
+    const bool more = kt + kStep < k1;
     const float flag = add;
     if (more) {
-      fetch(kt + TK);
-      masks(min(kt + 2 * TK, k1));
+      fetch(kt + kStep);
+      masks(min(kt + 2 * kStep, k1));
     }
     const L t(smem, buf);
-    if (active) {
+    if (active && kt < k1) {
       const int one = BIAS == kOrder ? far_entry(t.span(), span, a.rule.far) : -1;
       const float far_bias = one >= 0 ? lut[one] : 0.f;
       float far_sum = 0.f;
@@ -164,18 +171,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 ds[w][n][r] = power<M::kScaled, BIAS>(x[r], c, lut[e.i[r]], lse[n]) * (dp[r] - delta[n]);
-                hist[(wave * nb + lutb[e.i[r]]) * 64 + lane] += ds[w][n][r];
+                own[lutb[e.i[r]] * 64] += ds[w][n][r];
               }
             }
           }
         }
         M::template outer<NQ, false>(t.a + 32 * u * M::LD, ds[0], ds[1], dq, lane);
       }
-      if (BIAS == kOrder && one >= 0) hist[(wave * nb + lutb[one]) * 64 + lane] += far_sum;
+      if (BIAS == kOrder && one >= 0) own[lutb[one] * 64] += far_sum;
     }
-    if (more) put(buf ^ 1, kt + TK, flag);
+    if (more) put(buf ^ 1, kt + kStep, flag);
   }
-  if (active) {
+  if constexpr (KS > 1) {
+    __syncthreads();
+    float* image = (float*)(shared + wave * L::kBytes);
+    static_assert(M::DT * NQ * 1024 <= L::kBytes && KS == 2 && RW == 2, "a wave's sums fit a buffer");
+    if (active && group == 1) put_acc<NQ, M::DT>(image, dq, lane);
+    __syncthreads();
+    if (active && group == 0) add_acc<NQ, M::DT>(image, dq, lane);
+  }
+  if (active && group == 0) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int row = r0 + 16 * n + li;
@@ -185,7 +200,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
   }
   if constexpr (BIAS != kNoBias) {
     __syncthreads();
-    for (int b = wave; b < nb; b += 4) {
+    for (int b = threadIdx.x >> 6; b < nb; b += 4) {
       float t = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) t += hist[(w * nb + b) * 64 + lane];
@@ -196,7 +211,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
 }
 
 // The table's gradient: one wave adds the tiles' sums of one (head, bucket), in 64 bits and in order.
-__global__ __launch_bounds__(64) void bwd_table_kernel(const float* part, float* out, int tiles, int cells) {
+static __global__ __launch_bounds__(64) void bwd_table_kernel(const float* part, float* out, int tiles, int cells) {
   const int cell = blockIdx.x, lane = threadIdx.x;
   double t = 0.0;
   for (int i = lane; i < tiles; i += 64) t += (double)part[(int64_t)i * cells + cell];
@@ -205,15 +220,17 @@ __global__ __launch_bounds__(64) void bwd_table_kernel(const float* part, float*
 }
 
 // ------------------------------------------------------------------ key pass
-template <typename T, int DP, int NK, int BIAS, bool VEC>
+template <typename T, int DP, int NK, int BIAS, bool VEC, int RW, int KS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void bwd_key_kernel(Args a) {
   typedef Mat<T, DP> M;
   typedef Tiles<T, DP, 2> L;
-  constexpr int ROWS = 64 * NK, TK = L::TK;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  float* lut = (float*)(smem + 2 * L::kBytes);
+  constexpr int ROWS = 16 * NK * RW, NT = 64 * RW, TK = L::TK;
+  extern __shared__ __attribute__((aligned(16))) uint8_t shared[];
+  float* lut = (float*)(shared + KS * 2 * L::kBytes);
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, li = lane & 15;
+  const int tid = threadIdx.x % NT, lane = tid & 63, wave = tid >> 6, g = lane >> 4, li = lane & 15;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  uint8_t* smem = shared + group * 2 * L::kBytes;
   const int hk = blockIdx.x % a.Hk;
   const Tile tile = find_tile(a.k_ptr, a.S, a.Nk, ROWS, blockIdx.x / a.Hk);
   if (tile.start >= tile.end) return;
@@ -250,13 +267,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     }
   }
 
-  typedef Stage<T, DP, VEC> St;
+  typedef Stage<T, DP, VEC, NT> St;
   St sq, sd;
   typename St::Keep all;
   sq.init(a.q_row, a.D, tid);
   sd.init(a.do_row, a.D, tid);
   St::keep(all, nullptr, 0, 0, tid);
-  StagePos<BIAS, TK> sp;
+  StagePos<BIAS, TK, NT> sp;
   float row_lse = INFINITY, row_delta = 0.f;
   auto fetch = [&](int h, int qt) {
     sq.load((const T*)a.q + h * a.q_head, a.q_row, qt, q1 - qt, all, a.D, a.unit_q, tid);
@@ -279,23 +296,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
       t.f[TK + tid] = row_delta;
     }
   };
-  const int per = (q1 - q0 + TK - 1) / TK, steps = per * a.G;  // every query head of the group in turn
-  if (steps > 0) {
-    fetch(hk * a.G, q0);
-    put(0, q0);
+  // every query head of the group in turn, its tiles by KS at a time
+  const int per = (q1 - q0 + KS * TK - 1) / (KS * TK), steps = per * a.G;
+  auto tile_of = [&](int i) { return q0 + (i % per * KS + group) * TK; };
+  if (steps > 0 && tile_of(0) < q1) {
+    fetch(hk * a.G, tile_of(0));
+    put(0, tile_of(0));
   }
   for (int i = 0; i < steps; ++i) {
     const int h = hk * a.G + i / per;
     if (BIAS != kNoBias && i % per == 0) {
       __syncthreads();  // the head before is done with the look-up table
       const float* tab = (const float*)a.table + h * a.rule.buckets;
-      for (int j = tid; j < lut_size<BIAS>(a.rule); j += 256) lut[j] = tab[lut_bucket<BIAS>(a.rule, j)] * kLog2e;
+      for (int j = threadIdx.x; j < lut_size<BIAS>(a.rule); j += 256)
+        lut[j] = tab[lut_bucket<BIAS>(a.rule, j)] * kLog2e;
     }
     __syncthreads();
-    const bool more = i + 1 < steps;
-    if (more) fetch(hk * a.G + (i + 1) / per, q0 + (i + 1) % per * TK);
+    const bool more = i + 1 < steps && tile_of(i + 1) < q1;
+    if (more) fetch(hk * a.G + (i + 1) / per, tile_of(i + 1));
     const L t(smem, i & 1);
-    if (active) {
+    if (active && tile_of(i) < q1) {
       const int one = BIAS == kOrder ? far_entry(span, t.span(), a.rule.far) : -1;
       const float far_bias = one >= 0 ? lut[one] : 0.f;
 #pragma unroll
@@ -328,7 +348,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
         M::template outer<NK, false>(t.a + 32 * u * M::LD, ds[0], ds[1], dk, lane);
       }
     }
-    if (more) put((i + 1) & 1, q0 + (i + 1) % per * TK);
+    if (more) put((i + 1) & 1, tile_of(i + 1));
+  }
+  if constexpr (KS > 1) {
+    __syncthreads();
+    float* image = (float*)(shared + wave * 2 * L::kBytes);
+    static_assert(2 * M::DT * NK * 1024 <= 2 * L::kBytes && KS == 2 && RW == 2, "a wave's sums fit two buffers");
+    if (active && group == 1) {
+      put_acc<NK, M::DT>(image, dk, lane);
+      put_acc<NK, M::DT>(image + M::DT * NK * 256, dv, lane);
+    }
+    __syncthreads();
+    if (group == 1) return;
+    if (active) {
+      add_acc<NK, M::DT>(image, dk, lane);
+      add_acc<NK, M::DT>(image + M::DT * NK * 256, dv, lane);
+    }
   }
   if (!active) return;
 #pragma unroll
@@ -343,28 +378,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
 }
 
 // ------------------------------------------------------------------ host
-// Rows of a wave of the query pass: 32 in 16 bits, so that a fragment read from LDS feeds two
-// products, where that leaves two workgroups a compute unit; 16 with distances, whose arithmetic wants
-// the registers.  The key pass holds two accumulators a row and keeps to 16, but for narrow heads.
-static int wave_rows(at::ScalarType t, int bias, int64_t N, int64_t S, int64_t heads) {
-  if (t == at::kFloat || bias == kSpace) return 1;
-  (void)S;
-  return N / 128 * heads >= (bias == kOrder ? 2 : 8) * num_cus() ? 2 : 1;
-}
-
-int64_t table_tiles(const Args& a, at::ScalarType t, int bias) {
-  return tile_count(a.Nq, a.S, 64 * wave_rows(t, bias, a.Nq, a.S, a.H));
-}
-
-template <typename T, int DP, int NQ, int BIAS>
+template <typename T, int DP, int NQ, int BIAS, bool VEC, int RW>
 static void launch_query(const Args& a, float* dtable, hipStream_t st) {
-  const int nl = BIAS == kOrder ? 2 * a.rule.far + 1 : BIAS == kSpace ? a.rule.far + 1 : 0;
-  const int64_t qt = tile_count(a.Nq, a.S, 64 * NQ);
+  constexpr int KS = 4 / RW;
+  const int64_t qt = tile_count(a.Nq, a.S, 16 * NQ * RW);
   HY_CHECK(qt * a.H < (int64_t(1) << 31), "cross_attention: too many tiles for one launch");
-  size_t lds = 2 * Tiles<T, DP, 1>::kBytes;
-  if (BIAS != kNoBias) lds += 4 * a.rule.buckets * 64 * 4 + nl * 5;
-  auto* kern = a.unit_k == 16 && a.unit_v == 16 ? &bwd_query_kernel<T, DP, NQ, BIAS, true>
-                                                : &bwd_query_kernel<T, DP, NQ, BIAS, false>;
+  const size_t lds = KS * 2 * Tiles<T, DP, 1>::kBytes + table_bytes(a, BIAS, true);
+  auto* kern = &bwd_query_kernel<T, DP, NQ, BIAS, VEC, RW, KS>;
   allow_lds((const void*)kern, lds);
   kern<<<dim3((unsigned)(qt * a.H)), 256, lds, st>>>(a);
   if (BIAS != kNoBias) {
@@ -373,26 +393,33 @@ static void launch_query(const Args& a, float* dtable, hipStream_t st) {
   }
 }
 
-template <typename T, int DP, int NK, int BIAS>
+template <typename T, int DP, int NK, int BIAS, bool VEC, int RW>
 static void launch_key(const Args& a, hipStream_t st) {
-  const int nl = BIAS == kOrder ? 2 * a.rule.far + 1 : BIAS == kSpace ? a.rule.far + 1 : 0;
-  const int64_t kt = tile_count(a.Nk, a.S, 64 * NK);
+  constexpr int KS = 4 / RW;
+  const int64_t kt = tile_count(a.Nk, a.S, 16 * NK * RW);
   HY_CHECK(kt * a.Hk < (int64_t(1) << 31), "cross_attention: too many tiles for one launch");
-  const size_t lds = 2 * Tiles<T, DP, 2>::kBytes + nl * 4;
-  auto* kern = a.unit_q == 16 && a.unit_do == 16 ? &bwd_key_kernel<T, DP, NK, BIAS, true>
-                                                 : &bwd_key_kernel<T, DP, NK, BIAS, false>;
+  const size_t lds = KS * 2 * Tiles<T, DP, 2>::kBytes + table_bytes(a, BIAS, false);
+  auto* kern = &bwd_key_kernel<T, DP, NK, BIAS, VEC, RW, KS>;
   allow_lds((const void*)kern, lds);
   kern<<<dim3((unsigned)(kt * a.Hk)), 256, lds, st>>>(a);
 }
 
 template <typename T, int DP, int BIAS>
 static void launch_bwd(const Args& a, at::ScalarType t, float* dtable, hipStream_t st) {
-  constexpr int N2 = sizeof(T) == 2 && BIAS != kSpace ? 2 : 1;
-  if (wave_rows(t, BIAS, a.Nq, a.S, a.H) == 1) launch_query<T, DP, 1, BIAS>(a, dtable, st);
-  else launch_query<T, DP, N2, BIAS>(a, dtable, st);
-  constexpr int K2 = DP <= 32 ? N2 : 1;
-  if (wave_rows(t, BIAS, a.Nk, a.S, a.Hk) == 1) launch_key<T, DP, 1, BIAS>(a, st);
-  else launch_key<T, DP, K2, BIAS>(a, st);
+  constexpr int N2 = sizeof(T) == 2 && BIAS != kSpace ? 2 : 1, K2 = DP <= 32 ? N2 : 1;
+  const Form q = query_form(a, t, BIAS), k = key_form(a, t, BIAS);
+  const bool vec_q = a.unit_k == 16 && a.unit_v == 16, vec_k = a.unit_q == 16 && a.unit_do == 16;
+  constexpr int W2 = BIAS == kNoBias ? 2 : 4;
+  if (!vec_q && q.waves == 2) launch_query<T, DP, 1, BIAS, false, W2>(a, dtable, st);
+  else if (!vec_q) launch_query<T, DP, 1, BIAS, false, 4>(a, dtable, st);
+  else if (q.waves == 2) launch_query<T, DP, 1, BIAS, true, W2>(a, dtable, st);
+  else if (q.per == 2) launch_query<T, DP, N2, BIAS, true, 4>(a, dtable, st);
+  else launch_query<T, DP, 1, BIAS, true, 4>(a, dtable, st);
+  if (!vec_k && k.waves == 2) launch_key<T, DP, 1, BIAS, false, 2>(a, st);
+  else if (!vec_k) launch_key<T, DP, 1, BIAS, false, 4>(a, st);
+  else if (k.waves == 2) launch_key<T, DP, 1, BIAS, true, 2>(a, st);
+  else if (k.per == 2) launch_key<T, DP, K2, BIAS, true, 4>(a, st);
+  else launch_key<T, DP, 1, BIAS, true, 4>(a, st);
 }
 
 template <typename T, int DP>
@@ -403,17 +430,11 @@ static void pick(const Args& a, at::ScalarType t, int bias, float* dtable, hipSt
 }
 
 template <typename T>
-static void pick_width(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st) {
+void backward_rows(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st) {
   if (sizeof(T) == 4 && a.D <= 16) pick<T, sizeof(T) == 4 ? 16 : 32>(a, t, bias, dtable, st);
   else if (a.D <= 32) pick<T, 32>(a, t, bias, dtable, st);
   else if (a.D <= 64) pick<T, 64>(a, t, bias, dtable, st);
   else pick<T, 128>(a, t, bias, dtable, st);
-}
-
-void backward(const Args& a, at::ScalarType t, int bias, float* dtable, hipStream_t st) {
-  if (t == at::kFloat) pick_width<float>(a, t, bias, dtable, st);
-  else if (t == at::kBFloat16) pick_width<__bf16>(a, t, bias, dtable, st);
-  else pick_width<_Float16>(a, t, bias, dtable, st);
 }
 
 }  // namespace xa

@@ -1,0 +1,8 @@
+// The kernels of cross_attn_bwd.h for float.
+#include "cross_attn_bwd.h"
+
+namespace hy {
+namespace xa {
+template void backward_rows<float>(const Args&, at::ScalarType, int, float*, hipStream_t);
+}
+}  // namespace hy

@@ -1,21 +1,25 @@
 // Ragged cross attention, forward (see cross_attn.h for the mathematics and the layouts).
 //
-// A workgroup owns 64 NQ query rows of one sequence and one head; each of its four waves owns
-// 16 NQ of them and streams over all keys, whose tiles of 64 the workgroup stages in LDS once.
+// A workgroup owns 16 NQ RW query rows of one sequence and one head and streams over all keys, whose
+// tiles it stages in LDS, one ahead in registers; each of its waves owns 16 NQ of the rows.
+#pragma once
+
 #include "cross_attn.h"
 
 namespace hy {
 namespace xa {
 
-template <typename T, int DP, int NQ, int BIAS, bool SAVE, bool VEC>
+template <typename T, int DP, int NQ, int BIAS, bool SAVE, bool VEC, int RW, int KS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2 : 3))) void fwd_kernel(Args a) {
   typedef Mat<T, DP> M;
   typedef Tiles<T, DP, 1> L;
-  constexpr int ROWS = 64 * NQ, TK = L::TK, KB = TK / 16;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  float* lut = (float*)(smem + 2 * L::kBytes);
+  constexpr int ROWS = 16 * NQ * RW, NT = 64 * RW, TK = L::TK, KB = TK / 16;
+  extern __shared__ __attribute__((aligned(16))) uint8_t shared[];
+  float* lut = (float*)(shared + KS * 2 * L::kBytes);
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, li = lane & 15;
+  const int tid = threadIdx.x % NT, lane = tid & 63, wave = tid >> 6, g = lane >> 4, li = lane & 15;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  uint8_t* smem = shared + group * 2 * L::kBytes;
   const int h = blockIdx.x % a.H;
   const Tile tile = find_tile(a.q_ptr, a.S, a.Nq, ROWS, blockIdx.x / a.H);
   if (tile.start >= tile.end) return;
@@ -56,7 +60,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
   }
   if constexpr (BIAS != kNoBias) {
     const float* tab = (const float*)a.table + h * a.rule.buckets;
-    for (int i = tid; i < lut_size<BIAS>(a.rule); i += 256) lut[i] = tab[lut_bucket<BIAS>(a.rule, i)] * kLog2e;
+    for (int i = threadIdx.x; i < lut_size<BIAS>(a.rule); i += 256)
+      lut[i] = tab[lut_bucket<BIAS>(a.rule, i)] * kLog2e;
   }
 
   // s is an exponent of 2 where the scale or a bias is in it, else a product that c makes one
@@ -65,12 +70,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     return __builtin_amdgcn_exp2f(kDone ? s - top : fmaf(s, c, -top * c));
   };
 
-  typedef Stage<T, DP, VEC> St;
+  typedef Stage<T, DP, VEC, NT> St;
   St sk, sv;
   typename St::Keep keep;
   sk.init(a.k_row, a.D, tid);
   sv.init(a.v_row, a.D, tid);
-  StagePos<BIAS, TK> sp;
+  StagePos<BIAS, TK, NT> sp;
   auto fetch = [&](int kt) {  // a tile's rows, with the masks that the call before has fetched
     sk.load(k, a.k_row, kt, k1 - kt, keep, a.D, a.unit_k, tid);
     sv.load(v, a.v_row, kt, k1 - kt, keep, a.D, a.unit_v, tid);
@@ -88,23 +93,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
     sp.store(t.pos, k1 - kt, tid);
     if (tid < TK) t.f[tid] = flag;
   };
-  if (k0 < k1) {
-    masks(k0);
-    fetch(k0);
-    put(0, k0, add);
-    masks(min(k0 + TK, k1));
+  constexpr int kStep = KS * TK;
+  int kt = k0 + group * TK;  // (a group may have a tile less than the first)
+  if (kt < k1) {
+    masks(kt);
+    fetch(kt);
+    put(0, kt, add);
+    masks(min(kt + kStep, k1));
   }
   int buf = 0;
-  for (int kt = k0; kt < k1; kt += TK, buf ^= 1) {
+  for (int first = k0; first < k1; first += kStep, kt += kStep, buf ^= 1) {
     __syncthreads();  // this tile is there, and every wave is done with the one before it
-    const bool more = kt + TK < k1;
+    const bool more = kt + kStep < k1;
     const float flag = add;
     if (more) {
-      fetch(kt + TK);
-      masks(min(kt + 2 * TK, k1));
+      fetch(kt + kStep);
+      masks(min(kt + 2 * kStep, k1));
     }
     const L t(smem, buf);
-    if (active) {
+    if (active && kt < k1) {
       f4 s[KB][NQ];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {  // a key's 0 or -inf is what its products are added to
@@ -171,13 +178,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
       for (int u = 0; u < TK / 32; ++u)
         M::template outer<NQ, SAVE>(t.b + 32 * u * M::LD, s[2 * u], s[2 * u + 1], o, lane);
     }
-    if (more) put(buf ^ 1, kt + TK, flag);
+    if (more) put(buf ^ 1, kt + kStep, flag);
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) l[n] = column_sum(l[n]);
+  if constexpr (KS > 1) {
+    __syncthreads();
+    float* image = (float*)(shared + wave * L::kBytes);
+    static_assert((M::DT * NQ * 256 + 32 * NQ) * 4 <= L::kBytes && KS == 2 && RW == 2, "a wave's sums fit a buffer");
+    float* ml = image + M::DT * NQ * 256;
+    if (active && group == 1) {
+      put_acc<NQ, M::DT>(image, o, lane);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+        if (g == 0) {
+          ml[32 * n + li] = m[n];
+          ml[32 * n + 16 + li] = l[n];
+        }
+    }
+    __syncthreads();
+    if (group == 1) return;
+    if (active) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const float m1 = ml[32 * n + li], top = fmaxf(m[n], m1), at = top == -INFINITY ? 0.f : top;
+        const float by0 = power(m[n], at), by1 = power(m1, at);
+        l[n] = l[n] * by0 + ml[32 * n + 16 + li] * by1;
+        m[n] = top;
+#pragma unroll
+        for (int d = 0; d < M::DT; ++d)
+          o[n][d] = o[n][d] * by0 + *reinterpret_cast<const f4*>(image + ((n * M::DT + d) * 64 + lane) * 4) * by1;
+      }
+    }
   }
   if (!active) return;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int row = tile.start + r0 + 16 * n + li;
-    const float sum = column_sum(l[n]);
+    const float sum = l[n];
     if (row < tile.end) {
       const int64_t at = ((int64_t)row * a.H + h) * a.D;
       M::store((T*)a.out + at, o[n], sum > 0.f || sum != sum ? 1.f / sum : 0.f, a.D, g,
@@ -189,45 +227,43 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
   }
 }
 
-template <typename T, int DP, int NQ, int BIAS>
+template <typename T, int DP, int NQ, int BIAS, bool SAVE, bool VEC, int RW>
 static void launch_fwd(const Args& a, hipStream_t st) {
-  const int64_t blocks = tile_count(a.Nq, a.S, 64 * NQ) * a.H;
+  constexpr int KS = 4 / RW;
+  const int64_t blocks = tile_count(a.Nq, a.S, 16 * NQ * RW) * a.H;
   HY_CHECK(blocks < (int64_t(1) << 31), "cross_attention: too many query tiles for one launch");
-  size_t lds = 2 * Tiles<T, DP, 1>::kBytes;
-  if (BIAS == kOrder) lds += (2 * a.rule.far + 1) * 4;
-  if (BIAS == kSpace) lds += (a.rule.far + 1) * 4;
-  const bool vec = a.unit_k == 16 && a.unit_v == 16;
-  auto* kern = a.lse != nullptr
-                   ? (vec ? &fwd_kernel<T, DP, NQ, BIAS, true, true> : &fwd_kernel<T, DP, NQ, BIAS, true, false>)
-                   : (vec ? &fwd_kernel<T, DP, NQ, BIAS, false, true> : &fwd_kernel<T, DP, NQ, BIAS, false, false>);
+  const size_t lds = KS * 2 * Tiles<T, DP, 1>::kBytes + table_bytes(a, BIAS, false);
+  auto* kern = &fwd_kernel<T, DP, NQ, BIAS, SAVE, VEC, RW, KS>;
   allow_lds((const void*)kern, lds);
   kern<<<dim3((unsigned)blocks), 256, lds, st>>>(a);
 }
 
-// 16 bits: 32 rows a wave, so that a key fragment read from LDS feeds two products, where that leaves
-// eight workgroups a compute unit to even out sequences of unlike length; else 16, as with distances,
-// whose arithmetic wants the registers.
+template <typename T, int DP, int BIAS, bool SAVE>
+static void pick_form(const Args& a, at::ScalarType t, hipStream_t st) {
+  constexpr int N2 = sizeof(T) == 2 && BIAS != kSpace ? 2 : 1;
+  const Form f = forward_form(a, t, BIAS);
+  const bool vec = a.unit_k == 16 && a.unit_v == 16;
+  if (!vec && f.waves == 2) launch_fwd<T, DP, 1, BIAS, SAVE, false, 2>(a, st);
+  else if (!vec) launch_fwd<T, DP, 1, BIAS, SAVE, false, 4>(a, st);
+  else if (f.waves == 2) launch_fwd<T, DP, 1, BIAS, SAVE, true, 2>(a, st);
+  else if (f.per == 2) launch_fwd<T, DP, N2, BIAS, SAVE, true, 4>(a, st);
+  else launch_fwd<T, DP, 1, BIAS, SAVE, true, 4>(a, st);
+}
+
 template <typename T, int DP>
-static void pick(const Args& a, int bias, hipStream_t st) {
-  constexpr int N2 = sizeof(T) == 2 ? 2 : 1;
-  const bool two = N2 == 2 && (int64_t)(a.Nq / 128) * a.H >= 8 * num_cus();
-  if (bias == kNoBias) two ? launch_fwd<T, DP, N2, kNoBias>(a, st) : launch_fwd<T, DP, 1, kNoBias>(a, st);
-  else if (bias == kOrder) two ? launch_fwd<T, DP, N2, kOrder>(a, st) : launch_fwd<T, DP, 1, kOrder>(a, st);
-  else launch_fwd<T, DP, 1, kSpace>(a, st);
+static void pick(const Args& a, at::ScalarType t, int bias, hipStream_t st) {
+  const bool save = a.lse != nullptr;
+  if (bias == kNoBias) save ? pick_form<T, DP, kNoBias, true>(a, t, st) : pick_form<T, DP, kNoBias, false>(a, t, st);
+  else if (bias == kOrder) save ? pick_form<T, DP, kOrder, true>(a, t, st) : pick_form<T, DP, kOrder, false>(a, t, st);
+  else save ? pick_form<T, DP, kSpace, true>(a, t, st) : pick_form<T, DP, kSpace, false>(a, t, st);
 }
 
 template <typename T>
-static void pick_width(const Args& a, int bias, hipStream_t st) {
-  if (sizeof(T) == 4 && a.D <= 16) pick<T, sizeof(T) == 4 ? 16 : 32>(a, bias, st);
-  else if (a.D <= 32) pick<T, 32>(a, bias, st);
-  else if (a.D <= 64) pick<T, 64>(a, bias, st);
-  else pick<T, 128>(a, bias, st);
-}
-
-void forward(const Args& a, at::ScalarType t, int bias, hipStream_t st) {
-  if (t == at::kFloat) pick_width<float>(a, bias, st);
-  else if (t == at::kBFloat16) pick_width<__bf16>(a, bias, st);
-  else pick_width<_Float16>(a, bias, st);
+void forward_rows(const Args& a, at::ScalarType t, int bias, hipStream_t st) {
+  if (sizeof(T) == 4 && a.D <= 16) pick<T, sizeof(T) == 4 ? 16 : 32>(a, t, bias, st);
+  else if (a.D <= 32) pick<T, 32>(a, t, bias, st);
+  else if (a.D <= 64) pick<T, 64>(a, t, bias, st);
+  else pick<T, 128>(a, t, bias, st);
 }
 
 }  // namespace xa
