@@ -30,8 +30,8 @@ from ..ops.norm import norm_add
 from ..utils import tracer as tr
 from ..utils.model import activation_function_selection, loss_function_selection
 from ..utils.print_utils import print_master
-from .gps import GPSConv
-from .layers import BatchNorm, Ctx, Linear
+from .gps import GPSConv, attn_bias_buckets
+from .layers import AttentionPooling, BatchNorm, Ctx, GroupNorm, Linear, node_ptr
 
 
 class Base(nn.Module):
@@ -39,13 +39,16 @@ class Base(nn.Module):
     # False for stacks whose forward has data-dependent shapes (in-forward radius graphs,
     # triplet lists): the training engine then runs them eagerly instead of in a hipGraph
     capturable = True
+    # False for stacks whose decoder reads no pooled node features (MACE's read-outs)
+    pools_nodes = True
 
     def __init__(self, input_args="", conv_args="", input_dim=1, hidden_dim=8, output_dim=(1,), pe_dim=0,
                  global_attn_engine=None, global_attn_type=None, global_attn_heads=0, output_type=("graph",),
                  config_heads=None, activation_function_type="relu", loss_function_type="mse",
                  equivariance=False, ilossweights_hyperp=1, loss_weights=(1.0,), ilossweights_nll=0,
                  freeze_conv=False, initial_bias=None, dropout=0.25, num_conv_layers=16, num_nodes=None,
-                 attn_scope="batch"):
+                 attn_scope="batch", attn_bias=None, feature_norm="batch", feature_norm_groups=8,
+                 graph_pooling="mean", graph_pooling_heads=1):
         super().__init__()
         self.input_args = input_args
         self.conv_args = conv_args
@@ -72,6 +75,15 @@ class Base(nn.Module):
         self.batch_norms_node_output = ModuleDict({})
         self.equivariance = equivariance
         self.attn_scope = attn_scope
+        self.attn_bias = attn_bias_buckets(attn_bias)
+        if self.attn_bias is not None and not (global_attn_engine == "GPS" and attn_scope == "graph"):
+            raise ValueError("global_attn_bias needs global_attn_engine 'GPS' and global_attn_scope 'graph': "
+                             "distances between graphs mean nothing")
+        if feature_norm not in ("batch", "group"):
+            raise ValueError(f"feature_norm must be 'batch' or 'group', got {feature_norm!r}")
+        if graph_pooling not in ("mean", "attention"):
+            raise ValueError(f"graph_pooling must be 'mean' or 'attention', got {graph_pooling!r}")
+        self.feature_norm, self.feature_norm_groups = feature_norm, feature_norm_groups
         self.activation_function_type = activation_function_type
         self.activation_function = activation_function_selection(activation_function_type)
         self.var_output = 1 if loss_function_type == "GaussianNLLLoss" else 0
@@ -108,9 +120,16 @@ class Base(nn.Module):
         self.freeze_conv = freeze_conv
         self.initial_bias = initial_bias
         self._init_conv()
+        if feature_norm == "group" and not any(isinstance(n, GroupNorm) for n in self.feature_layers):
+            raise ValueError(f"{self}: no norm between its layers that feature_norm could choose")
         if freeze_conv:
             self._freeze_conv()
         self._multihead()
+        self.graph_pooling = None
+        if graph_pooling == "attention":
+            if "graph" not in self.head_type or not self.pools_nodes:
+                raise ValueError(f"{self}: no graph head that graph_pooling 'attention' could serve")
+            self.graph_pooling = AttentionPooling(hidden_dim, graph_pooling_heads)
         if initial_bias is not None:
             self._set_bias()
         self.conv_checkpointing = False
@@ -123,17 +142,20 @@ class Base(nn.Module):
     def _apply_global_attn(self, mpnn):
         if self.use_global_attn and self.global_attn_engine == "GPS":
             return GPSConv(self.hidden_dim, mpnn, heads=self.global_attn_heads, dropout=self.global_attn_dropout,
-                           attn_type=self.global_attn_type or "multihead")
+                           attn_type=self.global_attn_type or "multihead", attn_bias=self.attn_bias)
         return mpnn
+
+    def _feature_norm(self, width):
+        return GroupNorm(self.feature_norm_groups, width) if self.feature_norm == "group" else BatchNorm(width)
 
     def _init_conv(self):
         self.graph_convs.append(
             self._apply_global_attn(self.get_conv(self.embed_dim, self.hidden_dim, edge_dim=self.edge_embed_dim)))
-        self.feature_layers.append(BatchNorm(self.hidden_dim))
+        self.feature_layers.append(self._feature_norm(self.hidden_dim))
         for _ in range(self.num_conv_layers - 1):
             self.graph_convs.append(
                 self._apply_global_attn(self.get_conv(self.hidden_dim, self.hidden_dim, edge_dim=self.edge_embed_dim)))
-            self.feature_layers.append(BatchNorm(self.hidden_dim))
+            self.feature_layers.append(self._feature_norm(self.hidden_dim))
 
     def _freeze_conv(self):
         for module in (self.graph_convs, self.feature_layers):
@@ -306,6 +328,14 @@ class Base(nn.Module):
             inv = _zero_rows(inv, keep)
         for conv, bn in zip(self.graph_convs, self.feature_layers):
             inv, equiv = self._run_conv(conv, inv, equiv, ctx)
+            if isinstance(bn, GroupNorm):
+                kind = {torch.nn.ReLU: "relu", torch.nn.SiLU: "silu"}.get(type(self.activation_function), "none")
+                inv = bn(inv, node_ptr(inv, ctx), kind)
+                if kind == "none":
+                    inv = self.activation_function(inv)
+                if keep is not None:
+                    inv = _zero_rows(inv, keep)
+                continue
             if isinstance(self.activation_function, torch.nn.ReLU) and isinstance(bn, BatchNorm):
                 # BN -> ReLU -> padding mask in one fused launch (ops.norm.norm_add)
                 inv = norm_add(inv, bn, ctx.get("num_valid"), relu=True, zero_pad=keep is not None)
@@ -439,6 +469,8 @@ class Base(nn.Module):
         gsi = ctx.graph_si
         if ctx.get("pooled") is not None:
             x_graph = ctx.pooled  # pooled by a fused encoder
+        elif self.graph_pooling is not None:
+            x_graph = self.graph_pooling(x, node_ptr(x, ctx))
         elif gsi is None:
             x_graph = x.mean(dim=0, keepdim=True)
         else:
@@ -594,7 +626,10 @@ class Base(nn.Module):
         _rng.advance(next(self.parameters()).device)
         x, equiv, ctx = self.encode(data)
         fused_enc = ctx.get("pooled") is not None  # the whole-encoder fused path pooled already
-        x_graph = ctx.pooled if fused_enc else seg.segment_mean(x, ctx.graph_si)
+        if self.graph_pooling is not None:
+            x_graph = self.graph_pooling(x, node_ptr(x, ctx))
+        else:
+            x_graph = ctx.pooled if fused_enc else seg.segment_mean(x, ctx.graph_si)
         if x_graph.shape[0] != G or x_graph.shape[1] != self.hidden_dim:
             raise RuntimeError("fused_train_loss: pooled features do not match the targets")
         loss, _ = _mlp.head_loss(x_graph, layers, target, mask, self.loss_function_type, side=fused_enc)

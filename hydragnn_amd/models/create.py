@@ -20,7 +20,9 @@ def create_model_config(config, verbosity=0, use_gpu=True):
         a.get("equivariance", False), a.get("correlation"), a.get("max_ell"), a.get("node_max_ell"),
         a.get("avg_num_neighbors"), t.get("conv_checkpointing", False), verbosity, use_gpu,
         attn_scope=a.get("global_attn_scope", "batch"), dropout=a.get("dropout", 0.25),
-        init_seed=a.get("init_seed", 0),
+        init_seed=a.get("init_seed", 0), attn_bias=a.get("global_attn_bias"),
+        feature_norm=a.get("feature_norm", "batch"), feature_norm_groups=a.get("feature_norm_groups", 8),
+        graph_pooling=a.get("graph_pooling", "mean"), graph_pooling_heads=a.get("graph_pooling_heads", 1),
     )
 
 
@@ -32,7 +34,8 @@ def create_model(mpnn_type, input_dim, hidden_dim, output_dim, pe_dim, global_at
                  out_emb_size=None, envelope_exponent=None, num_spherical=None, num_gaussians=None, num_filters=None,
                  radius=None, equivariance=False, correlation=None, max_ell=None, node_max_ell=None,
                  avg_num_neighbors=None, conv_checkpointing=False, verbosity=0, use_gpu=True, attn_scope="batch",
-                 dropout=0.25, init_seed=0):
+                 dropout=0.25, init_seed=0, attn_bias=None, feature_norm="batch", feature_norm_groups=8,
+                 graph_pooling="mean", graph_pooling_heads=1):
     timer = Timer("create_model")
     timer.start()
     torch.manual_seed(init_seed)  # reference seeds 0; "init_seed" is an extension key
@@ -43,7 +46,9 @@ def create_model(mpnn_type, input_dim, hidden_dim, output_dim, pe_dim, global_at
                   activation_function_type=activation_function, loss_function_type=loss_function_type,
                   equivariance=equivariance, loss_weights=task_weights, freeze_conv=freeze_conv,
                   initial_bias=initial_bias, num_conv_layers=num_conv_layers, num_nodes=num_nodes,
-                  attn_scope=attn_scope, dropout=dropout)
+                  attn_scope=attn_scope, dropout=dropout, attn_bias=attn_bias, feature_norm=feature_norm,
+                  feature_norm_groups=feature_norm_groups, graph_pooling=graph_pooling,
+                  graph_pooling_heads=graph_pooling_heads)
     from . import stacks
 
     if mpnn_type == "GIN":

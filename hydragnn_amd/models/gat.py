@@ -183,7 +183,7 @@ class GATStack(Base):
         for (din, concat), w in zip(dims, widths):
             self.graph_convs.append(self._apply_global_attn(
                 self.get_conv(din, self.hidden_dim, concat=concat, edge_dim=self.edge_embed_dim)))
-            self.feature_layers.append(BatchNorm(w))
+            self.feature_layers.append(self._feature_norm(w))
 
     def _init_node_conv(self):
         nodeconfiglist = self.config_heads["node"]

@@ -18,17 +18,22 @@ import torch.nn.functional as F
 from torch import nn
 
 from ..ops.attention import segment_attention
+from ..ops.cross_attention import RelativeBuckets, cross_attention
 from ..ops.linear import ACT_RELU, linear
 from ..ops.norm import norm_add
 from ..ops.rng import dropout as rng_dropout, new_salt
 from ..ops.streams import Fork
 
 _GPS_FORK = os.environ.get("HYDRA_GPS_FORK", "1") == "1"  # attention branch on a side stream
-from .layers import BatchNorm, Linear
+from .layers import BatchNorm, Linear, node_ptr
 
 
 class MultiheadAttention(nn.Module):
-    def __init__(self, embed_dim, num_heads, bias=True):
+    """Self-attention over segments.  With ``rel_buckets`` (``ops.cross_attention.RelativeBuckets`` with
+    a unit) every score gets a learned bias by its pair's distance, ``rel_bias[head, bucket]``, and the
+    segments are the batch's graphs."""
+
+    def __init__(self, embed_dim, num_heads, bias=True, rel_buckets=None):
         super().__init__()
         assert embed_dim % num_heads == 0, "hidden_dim must be divisible by global_attn_heads"
         self.embed_dim = embed_dim
@@ -36,6 +41,9 @@ class MultiheadAttention(nn.Module):
         self.in_proj_weight = nn.Parameter(torch.empty(3 * embed_dim, embed_dim))
         self.in_proj_bias = nn.Parameter(torch.empty(3 * embed_dim)) if bias else None
         self.out_proj = Linear(embed_dim, embed_dim, bias=bias)
+        self.rel_buckets = rel_buckets
+        if rel_buckets is not None:  # zeros: it starts as the attention without a bias
+            self.rel_bias = nn.Parameter(torch.zeros(num_heads, rel_buckets.num_buckets))
         self._reset_parameters()
 
     def _reset_parameters(self):
@@ -44,9 +52,16 @@ class MultiheadAttention(nn.Module):
             nn.init.zeros_(self.in_proj_bias)
             nn.init.zeros_(self.out_proj.bias)
 
-    def forward(self, x, seg_id, seg_ptr):
+    def forward(self, x, seg_id, seg_ptr, pos=None):
         qkv = linear(x, self.in_proj_weight, self.in_proj_bias)
-        o = segment_attention(qkv, self.num_heads, seg_id, seg_ptr)
+        if self.rel_buckets is not None:
+            N, F = x.shape
+            q, k, v = qkv.view(N, 3, self.num_heads, F // self.num_heads).unbind(1)
+            pos = pos.detach().to(torch.float32)  # (a bucket has no slope in the positions)
+            o = cross_attention(q, k, v, seg_ptr, seg_ptr, table=self.rel_bias, buckets=self.rel_buckets, q_pos=pos,
+                                k_pos=pos).reshape(N, F)
+        else:
+            o = segment_attention(qkv, self.num_heads, seg_id, seg_ptr)
         return self.out_proj(o)
 
 
@@ -95,16 +110,37 @@ class PerformerAttention(nn.Module):
         return self.attn_out((num / den).reshape(N, H * D))
 
 
+def attn_bias_buckets(config):
+    """The buckets of the ``global_attn_bias`` entry of a configuration: None, or a dict with any of
+    ``num_buckets`` (32), ``max_distance`` (64, in units) and ``unit`` (0.25, in the positions' unit)."""
+    if not config:
+        return None
+    unknown = set(config) - {"num_buckets", "max_distance", "unit"}
+    if unknown:
+        raise ValueError(f"global_attn_bias: unknown entries {sorted(unknown)}")
+    return RelativeBuckets(config.get("num_buckets", 32), config.get("max_distance", 64),
+                           unit=config.get("unit", 0.25))
+
+
+def _positions(ctx):
+    if ctx.get("pos") is None:
+        raise ValueError("global_attn_bias needs node positions (data.pos)")
+    return ctx.pos
+
+
 class GPSConv(nn.Module):
-    def __init__(self, channels, conv, heads=1, dropout=0.0, act="relu", attn_type="multihead", norm=True):
+    def __init__(self, channels, conv, heads=1, dropout=0.0, act="relu", attn_type="multihead", norm=True,
+                 attn_bias=None):
         super().__init__()
         self.channels = channels
         self.conv = conv
         self.heads = heads
         self.dropout = dropout
         self.attn_type = attn_type or "multihead"
+        if attn_bias is not None and self.attn_type != "multihead":
+            raise ValueError(f"global_attn_bias needs global_attn_type 'multihead', got {self.attn_type!r}")
         if self.attn_type == "multihead":
-            self.attn = MultiheadAttention(channels, heads)
+            self.attn = MultiheadAttention(channels, heads, rel_buckets=attn_bias)
         elif self.attn_type == "performer":
             self.attn = PerformerAttention(channels, heads)
         else:
@@ -130,7 +166,10 @@ class GPSConv(nn.Module):
         # the attention branch runs on a side stream, concurrently with the local MPNN
         # (forward AND backward; ops/streams.py)
         with Fork(inv, ctx.attn_seg_id, ctx.attn_seg_ptr, enable=_GPS_FORK) as fork:
-            h = self.attn(inv, ctx.attn_seg_id, ctx.attn_seg_ptr)
+            if getattr(self.attn, "rel_buckets", None) is not None:
+                h = self.attn(inv, None, node_ptr(inv, ctx), _positions(ctx))
+            else:
+                h = self.attn(inv, ctx.attn_seg_id, ctx.attn_seg_ptr)
             h_att = norm_add(h, self.norm2, nv, residual=inv, p=self.dropout, salt=self._salts[1], training=tr)
         if self.conv is not None:
             h, equiv = self.conv(inv, equiv, ctx)

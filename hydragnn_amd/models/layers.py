@@ -40,6 +40,60 @@ class BatchNorm(nn.Module):
         return f"{self.__class__.__name__}({self.in_channels})"
 
 
+def node_ptr(x, ctx):
+    """CSR pointers (int32) of the batch's graphs over its node rows; one graph if it has none."""
+    si = ctx.get("graph_si")
+    if si is not None:
+        return si.rowptr
+    return torch.tensor([0, x.shape[0]], dtype=torch.int32, device=x.device)
+
+
+class GroupNorm(nn.Module):
+    """Group norm over the rows of each graph (``ops.norm.group_norm``): unlike ``BatchNorm``, a graph's
+    features do not depend on the rest of its batch, in training or after it."""
+
+    def __init__(self, groups, in_channels, eps=1e-5):
+        super().__init__()
+        if in_channels % groups:
+            raise ValueError(f"GroupNorm: {groups} groups do not divide {in_channels} channels")
+        self.groups, self.in_channels, self.eps = groups, in_channels, eps
+        self.weight = nn.Parameter(torch.ones(in_channels))
+        self.bias = nn.Parameter(torch.zeros(in_channels))
+
+    def forward(self, x, ptr, act="none"):
+        from ..ops.norm import group_norm
+
+        return group_norm(x, self.groups, self.weight, self.bias, ptr=ptr, eps=self.eps, act=act)
+
+    def __repr__(self):
+        return f"{self.__class__.__name__}({self.groups}, {self.in_channels})"
+
+
+class AttentionPooling(nn.Module):
+    """Read-out of each graph by learned queries that attend to its nodes (``ops.cross_attention``):
+    node rows [N, F] -> [graphs, F].  A graph without nodes reads zeros."""
+
+    def __init__(self, channels, heads, queries=1):
+        super().__init__()
+        if heads < 1 or channels % heads:
+            raise ValueError(f"AttentionPooling: {heads} heads do not divide {channels} channels")
+        if queries < 1:
+            raise ValueError(f"AttentionPooling: at least one query, got {queries}")
+        self.channels, self.heads, self.num_queries = channels, heads, queries
+        self.queries = nn.Parameter(torch.randn(queries, channels) / channels ** 0.5)
+        self.kv = Linear(channels, 2 * channels)
+        self.out = Linear(queries * channels, channels)
+
+    def forward(self, x, ptr):
+        from ..ops.cross_attention import cross_attention
+
+        G, T, H, D = ptr.numel() - 1, self.num_queries, self.heads, self.channels // self.heads
+        k, v = self.kv(x).view(x.shape[0], 2, H, D).unbind(1)
+        q = self.queries.to(x.dtype).expand(G, T, self.channels).reshape(G * T, H, D)
+        q_ptr = torch.arange(0, (G + 1) * T, T, dtype=torch.int32, device=x.device)
+        return self.out(cross_attention(q, k, v, q_ptr, ptr).reshape(G, T * self.channels))
+
+
 class Ctx:
     """Per-batch message-passing context handed to every conv layer."""
 

@@ -576,6 +576,7 @@ def process_node_attributes(x, num_elements=NUM_ELEMENTS):
 
 
 class MACEStack(Base):
+    pools_nodes = False
     is_edge_model = True
 
 

@@ -82,6 +82,8 @@ def eligible(model, ctx):
     F = model.hidden_dim
     if F not in (32, 64) or model.conv_checkpointing:
         return False
+    if model.attn_bias is not None or model.graph_pooling is not None or model.feature_norm != "batch":
+        return False
     if not isinstance(model.activation_function, torch.nn.ReLU):
         return False
     from .radial import MAX_K, MAX_L
