@@ -38,15 +38,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
   uint8_t* smem = shared + group * 2 * L::kBytes;
   const int h = blockIdx.x % a.H;
-  const Tile tile = find_tile(a.q_ptr, a.S, a.Nq, ROWS, blockIdx.x / a.H);
+  const Job job = find_job(a.q_ptr, a.Nq, a.k_ptr, a.Nk, a.S, ROWS, blockIdx.x / a.H);
+  const Tile tile = job.tile;
+  const int k0 = job.from, k1 = job.to;
   if (tile.start >= tile.end) {
     if (BIAS != kNoBias && (int)threadIdx.x < nb) a.part[(int64_t)blockIdx.x * nb + threadIdx.x] = 0.f;
     return;
-  }
-  int k0 = 0, k1 = 0;
-  if (tile.seq >= 0) {
-    k0 = min(max(a.k_ptr[tile.seq], 0), a.Nk);
-    k1 = min(max(a.k_ptr[tile.seq + 1], k0), a.Nk);
   }
   const T* k = (const T*)a.k + (h / a.G) * a.k_head;
   const T* v = (const T*)a.v + (h / a.G) * a.v_head;
@@ -232,13 +229,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
   uint8_t* smem = shared + group * 2 * L::kBytes;
   const int hk = blockIdx.x % a.Hk;
-  const Tile tile = find_tile(a.k_ptr, a.S, a.Nk, ROWS, blockIdx.x / a.Hk);
+  const Job job = find_job(a.k_ptr, a.Nk, a.q_ptr, a.Nq, a.S, ROWS, blockIdx.x / a.Hk);
+  const Tile tile = job.tile;
+  const int q0 = job.from, q1 = job.to;
   if (tile.start >= tile.end) return;
-  int q0 = 0, q1 = 0;
-  if (tile.seq >= 0) {
-    q0 = min(max(a.q_ptr[tile.seq], 0), a.Nq);
-    q1 = min(max(a.q_ptr[tile.seq + 1], q0), a.Nq);
-  }
   const int r0 = wave * 16 * NK, rows = tile.end - tile.start;
   const bool active = r0 < rows;
   typename M::Row kf[NK], vf[NK];

@@ -32,13 +32,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 64 ? 2
   const int h0 = hk * a.G + b % a.chunks * a.pack, heads = min(a.pack, a.G - b % a.chunks * a.pack);
   b /= a.chunks;
   const int sp = b % a.split;
-  const Tile tile = find_tile(a.q_ptr, a.S, a.Nq, a.rows, b / a.split);
+  const Job job = find_job(a.q_ptr, a.Nq, a.k_ptr, a.Nk, a.S, a.rows, b / a.split);
+  const Tile tile = job.tile;
+  const int k0 = job.from, k1 = job.to;
   if (tile.start >= tile.end) return;
-  int k0 = 0, k1 = 0;
-  if (tile.seq >= 0) {
-    k0 = min(max(a.k_ptr[tile.seq], 0), a.Nk);
-    k1 = min(max(a.k_ptr[tile.seq + 1], k0), a.Nk);
-  }
   const T* k = (const T*)a.k + hk * a.k_head;
   const T* v = (const T*)a.v + hk * a.v_head;
   T* own = (T*)smem + wave * kOwn;
