@@ -76,10 +76,12 @@ static int fill(Args& a, const at::Tensor& q, const at::Tensor& k, const at::Ten
   a.key_mask = nullptr;
   if (mask.has_value()) {
     HY_CHECK(mask->device() == dev && mask->scalar_type() == at::kBool && mask->is_contiguous() &&
-                 mask->numel() == k.size(0),
+                 mask->dim() == 1 && mask->numel() == k.size(0),
              "cross_attention: key_mask must be a contiguous bool for each key row");
     a.key_mask = (const uint8_t*)mask->data_ptr();
   }
+  HY_CHECK(table.has_value() == !rule.empty() && (table.has_value() || (!q_pos.has_value() && !k_pos.has_value())),
+           "cross_attention: a table, buckets and positions go together");
   if (!table.has_value()) return kNoBias;
   HY_CHECK(q_pos.has_value() && k_pos.has_value(), "cross_attention: a table needs q_pos and k_pos");
   const int bias = unit > 0 ? kSpace : kOrder;
@@ -90,7 +92,8 @@ static int fill(Args& a, const at::Tensor& q, const at::Tensor& k, const at::Ten
            "cross_attention: table must be contiguous fp32 [heads, buckets]");
   HY_CHECK(q_pos->device() == dev && k_pos->device() == dev && q_pos->scalar_type() == pt &&
                k_pos->scalar_type() == pt && q_pos->is_contiguous() && k_pos->is_contiguous() &&
-               q_pos->numel() == w * q.size(0) && k_pos->numel() == w * k.size(0),
+               q_pos->dim() == (w == 3 ? 2 : 1) && k_pos->dim() == q_pos->dim() && q_pos->size(0) == q.size(0) &&
+               k_pos->size(0) == k.size(0) && q_pos->numel() == w * q.size(0) && k_pos->numel() == w * k.size(0),
            "cross_attention: positions must be contiguous, int32 [rows] or fp32 [rows, 3]");
   HY_CHECK(rule.size() >= 4 && rule.size() <= 4 + kMaxBuckets, "cross_attention: bucket rule");
   Rule& r = a.rule;

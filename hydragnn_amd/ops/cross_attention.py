@@ -160,17 +160,22 @@ def cross_attention(q, k, v, q_ptr, k_ptr, scale=None, key_mask=None, table=None
     Pointers that do not ascend give unspecified outputs on the GPU (nothing outside the tensors
     is read or written) and raise on the CPU.  Differentiable once in q, k, v and table on the GPU.
     """
-    _check(q, k, v, q_ptr, k_ptr, key_mask, table, buckets, q_pos, k_pos)
-    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None else float(scale)
     if not q.is_cuda or not _mode.fused("attn"):
+        _check(q, k, v, q_ptr, k_ptr, key_mask, table, buckets, q_pos, k_pos)
         return cross_attention_reference(q, k, v, q_ptr, k_ptr, scale, key_mask, table, buckets, q_pos, k_pos)
     rule, unit = ([], 0.0) if buckets is None else (buckets.rule, buckets.unit or 0.0)
-    if table is not None:
-        table, q_pos, k_pos = table.float().contiguous(), q_pos.contiguous(), k_pos.contiguous()
-    if key_mask is not None:
-        key_mask = key_mask.contiguous()
-    q_ptr, k_ptr = q_ptr.contiguous(), k_ptr.contiguous()
-    return _native.ops().cross_attention(q, k, v, q_ptr, k_ptr, key_mask, scale, table, q_pos, k_pos, rule, unit)
+    tab, qp, kp = table, q_pos, k_pos
+    try:
+        if table is not None and q_pos is not None and k_pos is not None:
+            tab = table.float() if table.dtype == q.dtype else table
+            tab, qp, kp = tab.contiguous(), q_pos.contiguous(), k_pos.contiguous()
+        return _native.ops().cross_attention(q, k, v, q_ptr.contiguous(), k_ptr.contiguous(),
+                                             None if key_mask is None else key_mask.contiguous(), scale, tab, qp, kp,
+                                             rule, unit)
+    except (RuntimeError, TypeError):  # the operator refuses what _check refuses, which says why
+        _check(q, k, v, q_ptr, k_ptr, key_mask, table, buckets, q_pos, k_pos)
+        raise
 
 
 def _attend(q, k, v, scale, bias):

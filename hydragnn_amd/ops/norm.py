@@ -190,19 +190,20 @@ def group_norm(x, groups, weight=None, bias=None, ptr=None, eps=1e-5, act="none"
 
     Statistics are summed in 64 bits.  Differentiable once in x, weight and bias on the GPU.
     """
-    _check_group_norm(x, groups, weight, bias, ptr, act)
     if not x.is_cuda or not _mode.fused("norm"):
+        _check_group_norm(x, groups, weight, bias, ptr, act)
         return group_norm_reference(x, groups, weight, bias, ptr, eps, act)
-    shape = x.shape
-    seqs = 0
-    if ptr is None:
-        seqs = shape[0]
-        x = x.reshape(-1, shape[-1])
-    else:
-        ptr = ptr.contiguous()
-    w, b = (None if p is None else p.float().contiguous() for p in (weight, bias))
-    y = _native.ops().group_norm(x, w, b, ptr, seqs, groups, float(eps), _ACTS[act])
-    return y if y.shape == shape else y.view(shape)
+    try:
+        rows, seqs = x, 0
+        if ptr is None:
+            rows, seqs = x.reshape(-1, x.shape[-1]), x.shape[0]
+        w, b = (p.float() if p is not None and p.dtype == x.dtype else p for p in (weight, bias))
+        y = _native.ops().group_norm(rows, None if w is None else w.contiguous(), None if b is None else b.contiguous(),
+                                     None if ptr is None else ptr.contiguous(), seqs, groups, float(eps), _ACTS[act])
+    except (RuntimeError, TypeError, LookupError):  # the operator refuses what the check refuses, which says why
+        _check_group_norm(x, groups, weight, bias, ptr, act)
+        raise
+    return y if rows is x else y.view(x.shape)
 
 
 def group_norm_reference(x, groups, weight, bias, ptr, eps=1e-5, act="none"):

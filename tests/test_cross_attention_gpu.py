@@ -320,3 +320,20 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), q)
     assert HALF[torch.float32] == torch.finfo(torch.float32).eps / 2
+
+
+def _refused():
+    import test_cross_attention as cpu
+
+    for mark in cpu.test_refusals.pytestmark:
+        yield from (c for c in mark.args[1] if c[1] != "ascend")
+
+
+@pytest.mark.parametrize("change,what", list(_refused()))
+def test_the_gpu_refuses_what_the_cpu_refuses(change, what):
+    import test_cross_attention as cpu
+
+    q, k, v, _, qp, kp = cpu._inputs(dtype=torch.float32)
+    a = {"q": q, "k": k, "v": v, "q_ptr": qp, "k_ptr": kp, **change}
+    with pytest.raises(ValueError, match=what):
+        cross_attention(**{n: t.to(DEV) if torch.is_tensor(t) else t for n, t in a.items()})

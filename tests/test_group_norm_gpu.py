@@ -208,3 +208,17 @@ def test_refusals():
         group_norm(x, 2, torch.ones(8))
     with pytest.raises(ValueError, match="not supported"):
         group_norm(x.double(), 2)
+
+
+def _refused():
+    import test_group_norm as cpu
+
+    for mark in cpu.test_refusals.pytestmark:
+        yield from (c for c in mark.args[1] if c[1] != "ascend")
+
+
+@pytest.mark.parametrize("change,what", list(_refused()))
+def test_the_gpu_refuses_what_the_cpu_refuses(change, what):
+    a = {"x": torch.zeros(4, 8), "groups": 2, **change}
+    with pytest.raises(ValueError, match=what):
+        group_norm(**{n: t.to(DEV) if torch.is_tensor(t) else t for n, t in a.items()})
