@@ -29,9 +29,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // so the bare instruction is exact enough and -inf still maps to 0.
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Packed fp32 (v_pk_fma_f32 on gfx950): two lanes of math per VALU op.  The
-// D-wide dot products and rank-1 updates of the inner loops run on float2 pairs,
-// halving the FMA instruction count (the kernels are VALU-issue bound at D = 8).
+// The D-wide dot products and rank-1 updates of the inner loops run on float2 pairs.  (They were
+// written for packed fp32 arithmetic, which the build keeps off: some of its forms have given wrong
+// results without an error.  Every pair is two ordinary operations now.)
 typedef float f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f2 pfma(f2 a, f2 b, f2 c) { return __builtin_elementwise_fma(a, b, c); }
 __device__ __forceinline__ f2 splat2(float v) { return f2{v, v}; }
