@@ -614,7 +614,7 @@ static void forward(Args a, hipStream_t st, const at::TensorOptions& opt) {
     a.stat = stat.data_ptr<float>();
   }
   launch(&fwd_sums_kernel<T, VEC>, a.chunks, sums, st, a);
-  fwd_finish_kernel<<<dim3(a.S * ceil_div(a.G, 16)), 1024, 0, st>>>(a);
+  if (a.S > 0) fwd_finish_kernel<<<dim3(a.S * ceil_div(a.G, 16)), 1024, 0, st>>>(a);
   launch(&fwd_apply_kernel<T, ACT, VEC>, a.chunks, 0, st, a);
 }
 

@@ -115,11 +115,23 @@ def check_norm(got, ref, tol, what, floor=0.0):
     assert off <= tol * size + floor, f"{what}: off by {off:.3e} of {size:.3e} (tol {tol:.1e})"
 
 
-def check_table(got, res, dtype, what):
+def score_error(q, k, scale):
+    """Bound of a score's absolute error, where scores are not of the order of 1: a score is a sum of D
+    products, rounded D times by half a step of a partial sum, which is at most S = |scale| sum |q k|;
+    the errors are independent, so they add up to the root of D of them, and 4 more cover the scale's,
+    the bias' and the logarithm's.  p = exp(score - lse) is off by that much, relatively, once for the
+    score and once for the lse."""
+    g = q.shape[1] // k.shape[1]
+    kk = k.double().abs().repeat_interleave(g, 1).transpose(0, 1)
+    size = (q.double().abs().transpose(0, 1) @ kk.transpose(1, 2)).max().item() * abs(scale)
+    return 2 * (math.sqrt(q.shape[2]) + 4) * size * U32
+
+
+def check_table(got, res, dtype, what, p_error=0.0):
     """Every dS is off by its factors' roundings, (|dP| + |delta|) p times a few 2^-24, and in 16 bits
     by delta's: `out` and what its rounding leaves give 2 half steps squared, p in two parts as much."""
     h = HALF[dtype]
-    rel = 128 * U32 + (0 if dtype == torch.float32 else 4 * h * h)
+    rel = 128 * U32 + p_error + (0 if dtype == torch.float32 else 4 * h * h)
     off = (got.detach().double().cpu() - res["dtable"]).abs()
     bound = rel * res["dtable_size"] + 1e-30
     assert (off <= bound).all(), f"{what}: off by {(off / bound).max().item():.2f} of the bound"

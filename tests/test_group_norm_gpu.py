@@ -222,3 +222,32 @@ def test_the_gpu_refuses_what_the_cpu_refuses(change, what):
     a = {"x": torch.zeros(4, 8), "groups": 2, **change}
     with pytest.raises(ValueError, match=what):
         group_norm(**{n: t.to(DEV) if torch.is_tensor(t) else t for n, t in a.items()})
+
+
+def test_no_sequences():
+    """Every row lies behind the last sequence, whatever their number."""
+    for n in (5, 50000):
+        x = torch.randn(n, 32, device=DEV, requires_grad=True)
+        w = torch.ones(32, device=DEV, requires_grad=True)
+        out = group_norm(x, 4, w, ptr=_ptr([], DEV))
+        dx, dw = torch.autograd.grad(out, (x, w), torch.ones_like(out))
+        assert not out.any() and not dx.any() and not dw.any()
+
+
+def test_offsets_past_32_bits():
+    n, C = 530000, 4096  # 2.2e9 values: the last rows lie beyond 2^31 of them
+    x = torch.empty(n, C, device=DEV, dtype=torch.bfloat16)
+    x[-700:] = torch.randn(700, C, device=DEV).bfloat16()
+    x.requires_grad_()
+    ptr = torch.tensor([0, 0, 200], dtype=torch.int32, device=DEV) + (n - 700)
+    ptr[0] = 0  # the first sequence's rows hold whatever memory held: only the others are looked at
+    ptr = torch.cat([ptr, torch.tensor([n], dtype=torch.int32, device=DEV)])
+    out = group_norm(x, 32, ptr=ptr, act="silu")
+    small = x.detach()[-700:].clone().requires_grad_()
+    ref = group_norm(small, 32, ptr=_ptr([0, 200, 500], DEV), act="silu")
+    _off(out[-700:], ref.detach().double().cpu(), HALF[torch.bfloat16] + 64 * U32, "out")
+    dy = torch.zeros_like(out)
+    dy[-700:] = torch.randn(700, C, device=DEV).bfloat16()
+    (dx,) = torch.autograd.grad(out, x, dy)
+    (rx,) = torch.autograd.grad(ref, small, dy[-700:].clone())
+    _off(dx[-700:], rx.double().cpu(), HALF[torch.bfloat16] + 64 * U32, "dx")
